@@ -512,6 +512,138 @@ int mcTile(const float* bottom, float* top, long outer, int inner, int tiles, vo
 /* Fill `count` floats with `value` (caffe_gpu_set, math_functions.cu:70-82). */
 int mcFill(float* dst, long count, float value, void* stream);
 
+/* ---- attention of language models over image and text tokens ------------------ */
+/* No counterpart in the reference.  The cells of a feature map are tokens like those of
+ * a text; these operators serve a model that answers about images: bookkeeping of a
+ * paged cache, rotary positions, attention of whole prompts and over the cache.
+ * Forward only, as everything here. */
+
+/* Element types.  Sums, softmax statistics and angles are held in 32 bits for all. */
+enum mcDataType { MC_TYPE_F32 = 0, MC_TYPE_F16 = 1, MC_TYPE_BF16 = 2 };
+
+/* Rows of heads: head h of token t starts at element t * token_stride + h * head_stride
+ * of `data` (device), its head_dim values are contiguous.  `data` and both strides, in
+ * bytes, are multiples of 16.  One struct describes a slice of a fused projection, a
+ * plain [tokens, heads, head_dim] blob or a transposed one. */
+typedef struct mcHeads {
+  void* data;
+  long token_stride;
+  long head_stride;
+} mcHeads;
+
+/* A paged cache: slot s of a head is row s % block_size of block s / block_size, at
+ * element (s / block_size) * block_stride + (s % block_size) * token_stride +
+ * head * head_stride of `keys` and of `values` (device; 16-byte rule as above).
+ * num_blocks * block_size fits an int; the strides are 64-bit, so the memory may be
+ * larger.  A block number outside [0, num_blocks) is never followed: what it should
+ * hold is left out of an attention, and not stored. */
+typedef struct mcPagedCache {
+  void* keys;
+  void* values;
+  int num_blocks;
+  int block_size;
+  long block_stride, token_stride, head_stride;
+} mcPagedCache;
+
+/* Bookkeeping of a paged cache on the GPU, from the lengths of the requests.  Request r
+ * holds cached_lens[r] tokens and gets new_lens[r] more (0 allowed).  Blocks that its
+ * table lacks for them are taken from the end of free_blocks[0 .. *free_count), request
+ * by request.  Writes, all on the device:
+ *   block_table  [num_requests, table_width], the new entries only
+ *   context_lens [num_requests] cached + new
+ *   row_starts   [num_requests + 1] first new token of each request, packed
+ *   slots        [max_tokens] slot of each new token, -1 behind the last
+ *   positions    [max_tokens] its position in its request, 0 behind the last
+ *   free_left    blocks that stay free (*free_count and *free_left are not the same int:
+ *                pass them in turn; free_blocks itself is not changed)
+ *   denied       number of requests that got nothing: the pool was used up (by them or
+ *                by an earlier one that was denied; a request that needs no block is
+ *                served all the same), or the table is not wide enough.  Their tokens
+ *                have slot -1 and their context_lens entry is cached_lens[r].
+ * At most 4096 requests; max_tokens and free_capacity (the length of the free_blocks
+ * array) below 2^23 - 1.
+ * Nothing is read back, so the call can be captured. */
+int mcCacheReserve(int num_requests, int block_size, int table_width, int max_tokens,
+                   int free_capacity, const int* cached_lens, const int* new_lens,
+                   const int* free_blocks, const int* free_count, int* block_table,
+                   int* context_lens, int* row_starts, int* slots, int* positions,
+                   int* free_left, int* denied, void* stream);
+
+/* Gives the blocks of every request with finished[r] != 0 back: they are put behind
+ * free_blocks[0 .. *free_count) in request order, context_lens[r] becomes 0, and
+ * *free_left (may be free_count) the new count.  Blocks that would not fit into
+ * free_capacity entries are dropped. */
+int mcCacheRelease(int num_requests, int block_size, int table_width, int free_capacity,
+                   const int* finished, const int* block_table, int* context_lens,
+                   int* free_blocks, const int* free_count, int* free_left, void* stream);
+
+/* Rotary positions with up to four axes.  Pair i of a head (0 <= i < rotary_dim / 2) is
+ * turned by the angle positions[axis(i)][token] * frequencies[i], the product rounded to
+ * 32 bits as models are trained with it; its cosine and sine are exact to 32 bits at any
+ * size.  Pairs are (i, i + rotary_dim / 2), or neighbours (2i, 2i + 1) with `adjacent`.
+ * The axes share the pairs by sections[] (sum rotary_dim / 2): one section behind the
+ * other, or with `cycled` dealt out in turn (0, 1, 2, 0, 1, 2, ...) until a section's
+ * number is reached.  Values from rotary_dim on are copied. */
+typedef struct mcRotaryGeom {
+  int type;        /* enum mcDataType */
+  int heads;       /* query heads */
+  int heads_kv;    /* key and value heads; 0 = queries only */
+  int head_dim;    /* a multiple of 8, at most 256 */
+  int rotary_dim;  /* even, at most head_dim */
+  int adjacent;
+  int num_axes;    /* 1 to 4 */
+  int sections[4];
+  int cycled;
+} mcRotaryGeom;
+
+/* frequencies [rotary_dim / 2]; positions: axis a at positions + a * axis_stride, `tokens`
+ * ints each.  q -> q_out.  k (or NULL) -> k_out (or NULL) and, with a cache, the cache's
+ * keys at slots[token]; v (or NULL) -> the cache's values there, unchanged.  A slot
+ * outside the cache (-1: none) is not stored.  q_out == q and k_out == k are allowed
+ * (same strides). */
+int mcRotary(const mcRotaryGeom* geom, const float* frequencies, const int* positions,
+             long axis_stride, int tokens, const mcHeads* q, const mcHeads* q_out, const mcHeads* k,
+             const mcHeads* k_out, const mcHeads* v, const mcPagedCache* cache, const int* slots,
+             void* stream);
+
+/* out = softmax(scale * q k^T) v per head; query head h reads key head h / (heads /
+ * heads_kv).  causal: the last query of a sequence sees all of its keys, the one before
+ * one less, and so on (with as many queries as keys, each sees the keys up to its own).
+ * A query that sees no key, or only such with score -inf, gives zeros and -inf as its lse. */
+typedef struct mcAttentionGeom {
+  int type;      /* enum mcDataType of all operands */
+  int heads;     /* query heads, a multiple of heads_kv */
+  int heads_kv;
+  int head_dim;  /* a multiple of 8, at most 256 */
+  int causal;
+  float scale;   /* positive */
+} mcAttentionGeom;
+
+/* Attention of packed sequences: sequence s has the queries q_starts[s] .. q_starts[s+1]
+ * and the keys and values k_starts[s] .. k_starts[s+1] (device, num_sequences + 1 ints
+ * each, ascending; the same array for self-attention).  total_q / total_k: rows of q / of
+ * k and v.  lse [heads, total_q] (or NULL) gets the natural logarithm of the sum of
+ * exp(scale * q k).  What other sequences hold, NaN and infinities included, does not
+ * reach a row, nor do values at keys that it does not see.  out overlaps no input. */
+int mcAttentionPacked(const mcAttentionGeom* geom, const mcHeads* q, const mcHeads* k,
+                      const mcHeads* v, const int* q_starts, const int* k_starts,
+                      int num_sequences, int total_q, int total_k, const mcHeads* out, float* lse,
+                      void* stream);
+
+/* Attention of new tokens over a paged cache that holds them already (mcRotary stores
+ * them): request r has the queries q_starts[r] .. q_starts[r+1] and context_lens[r] keys,
+ * key j in block block_table[r * table_width + j / block_size].  One new token per
+ * request (a step of text), or a chunk of a prompt.  max_q / max_context: no request has
+ * more new tokens / keys (host numbers that size the launch; a request's rows beyond
+ * max_q are not computed, keys beyond max_context or the table not seen).  Work over a
+ * long context with few rows is cut into pieces; their partial results lie in scratch
+ * that the calling thread owns (mcReleaseScratch): before the call is captured, make one
+ * call of the same sizes outside. */
+int mcAttentionPaged(const mcAttentionGeom* geom, const mcHeads* q, const mcPagedCache* cache,
+                     const int* block_table, int table_width, const int* q_starts,
+                     const int* context_lens, int num_requests, int total_q, int max_q,
+                     int max_context, const mcHeads* out, float* lse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

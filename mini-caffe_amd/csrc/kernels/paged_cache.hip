@@ -1,0 +1,262 @@
+// Bookkeeping of a paged cache: block tables, slots and positions of new tokens from the
+// lengths of the requests, on the device.
+//
+//   have_r = ceil(cached_r / B), need_r = ceil((cached_r + new_r) / B),
+//   taken_r = sum over earlier requests of (need - have), starts_r = sum of their new_r,
+//   table[r][have_r + j] = free[count - 1 - taken_r - j],
+//   slot of token t of request r: table[r][p / B] * B + p % B at p = cached_r + t - starts_r.
+//
+// Kilobytes go in and out: what counts is the number of dependent steps.  One launch: every
+// workgroup forms the two prefix sums by itself in LDS (a few loads per thread, all from
+// the L2) and then writes its share of tokens, fresh blocks and requests, finding the
+// request of each by bisection.  A fresh block's number comes from the free list, never
+// from a table entry that another workgroup writes.
+#include "mc_common.h"
+#include "mchip/kernels.h"
+
+#include <algorithm>
+#include <climits>
+
+namespace mchip {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxRequests = 4096;  // two prefix sums of ints: 32 KiB of LDS
+constexpr int kMaxLength = 1 << 30;                // what a length is clipped to
+constexpr int kMaxCount = INT_MAX / kThreads;      // tokens of a call, blocks of a pool
+
+struct ReserveArgs {
+  int num, block, width, max_tokens, free_capacity;
+  const int* cached;
+  const int* fresh;
+  const int* free_blocks;
+  const int* free_count;
+  int* table;
+  int* contexts;
+  int* starts;
+  int* slots;
+  int* positions;
+  int* free_left;
+  int* denied;
+};
+
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Exclusive sum over a workgroup of kThreads; *total gets the sum of all.
+__device__ __forceinline__ int block_scan(int v, int* lds, int* total) {
+  const int wave = threadIdx.x >> 6;
+  const int incl = wave_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) lds[wave] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    if (w < wave) before += lds[w];
+    all += lds[w];
+  }
+  *total = all;
+  return before + incl - v;
+}
+
+// Sums stay in an int whatever the lengths hold: a request's are clipped, the sum over a
+// thread's run of requests saturates, and counts as kMaxCount at most in the sum over the
+// threads.  Whatever lies behind such a run then starts at kMaxCount or later, past the last
+// token and the last block there can be, so the bisections still see ascending sums below it.
+__device__ __forceinline__ int sat_add(int a, int b) {
+  const unsigned s = static_cast<unsigned>(a) + static_cast<unsigned>(b);
+  return s > static_cast<unsigned>(kMaxLength) ? kMaxLength : static_cast<int>(s);
+}
+
+struct Lengths {
+  int cached, fresh, have, more;
+  bool wide;  // the table has room for its blocks
+};
+__device__ __forceinline__ Lengths lengths_of(const ReserveArgs& a, int r) {
+  Lengths l;
+  l.cached = min(max(a.cached[r], 0), kMaxLength);
+  l.fresh = min(max(a.fresh[r], 0), kMaxLength);
+  l.have = static_cast<int>((static_cast<long>(l.cached) + a.block - 1) / a.block);
+  const int need = static_cast<int>((static_cast<long>(l.cached) + l.fresh + a.block - 1) / a.block);
+  l.wide = need <= a.width;
+  l.more = l.wide ? need - l.have : 0;
+  return l;
+}
+
+// Last index i in [0, n) with sums[i] <= v (sums ascending from 0).
+__device__ __forceinline__ int last_at_most(const int* sums, int n, int v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (sums[mid] <= v) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kThreads) void reserve_kernel(ReserveArgs a) {
+  extern __shared__ int lds[];
+  int* starts = lds;            // [num]
+  int* taken = lds + a.num;     // [num]
+  __shared__ int scan_lds[kThreads / 64];
+  const int tid = threadIdx.x;
+  const int have_free = min(max(a.free_count[0], 0), a.free_capacity);
+
+  // the two prefix sums, each thread over a run of requests
+  const int per = (a.num + kThreads - 1) / kThreads;
+  const int first = min(tid * per, a.num), last = min(first + per, a.num);
+  int tokens = 0, blocks = 0;
+  for (int r = first; r < last; ++r) {
+    const Lengths l = lengths_of(a, r);
+    tokens = sat_add(tokens, l.fresh);
+    blocks = sat_add(blocks, l.more);
+  }
+  int total_tokens, total_blocks;
+  int at_token = block_scan(min(tokens, kMaxCount), scan_lds, &total_tokens);
+  int at_block = block_scan(min(blocks, kMaxCount), scan_lds, &total_blocks);
+  for (int r = first; r < last; ++r) {
+    const Lengths l = lengths_of(a, r);
+    starts[r] = at_token;
+    taken[r] = at_block;
+    at_token = sat_add(at_token, l.fresh);
+    at_block = sat_add(at_block, l.more);
+  }
+  __syncthreads();
+
+  const int step = gridDim.x * kThreads, me = blockIdx.x * kThreads + tid;
+  // requests
+  int granted_end = 0, refused = 0;
+  for (int r = blockIdx.x == 0 ? tid : a.num; r < a.num; r += kThreads) {
+    const Lengths l = lengths_of(a, r);
+    const bool ok = l.wide && (l.more == 0 || taken[r] + l.more <= have_free);
+    a.contexts[r] = ok ? l.cached + l.fresh : l.cached;
+    a.starts[r] = starts[r];
+    if (ok && l.more) granted_end = max(granted_end, taken[r] + l.more);
+    refused += !ok;
+  }
+  if (blockIdx.x == 0) {
+    int all;
+    block_scan(refused, scan_lds, &all);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) granted_end = max(granted_end, __shfl_xor(granted_end, o, 64));
+    __syncthreads();
+    if ((tid & 63) == 0) scan_lds[tid >> 6] = granted_end;
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 1; w < kThreads / 64; ++w) granted_end = max(granted_end, scan_lds[w]);
+      a.free_left[0] = have_free - granted_end;
+      a.denied[0] = all;
+      a.starts[a.num] = total_tokens;
+    }
+  }
+  // fresh blocks
+  const int granted_blocks = min(total_blocks, have_free);
+  for (int f = me; f < granted_blocks; f += step) {
+    const int r = last_at_most(taken, a.num, f);
+    const Lengths l = lengths_of(a, r);
+    const int j = f - taken[r];
+    if (j < l.more && taken[r] + l.more <= have_free)
+      a.table[static_cast<long>(r) * a.width + l.have + j] = a.free_blocks[have_free - 1 - f];
+  }
+  // tokens
+  for (int t = me; t < a.max_tokens; t += step) {
+    int slot = -1, p = 0;
+    if (t < total_tokens) {
+      const int r = last_at_most(starts, a.num, t);
+      const Lengths l = lengths_of(a, r);
+      const int i = t - starts[r];
+      p = l.cached + i;
+      if (i < l.fresh && l.wide && (l.more == 0 || taken[r] + l.more <= have_free)) {
+        const int b = p / a.block;
+        const int number = b < l.have ? a.table[static_cast<long>(r) * a.width + b]
+                                      : a.free_blocks[have_free - 1 - taken[r] - (b - l.have)];
+        slot = number < 0 ? -1 : number * a.block + p % a.block;
+      }
+    }
+    a.slots[t] = slot;
+    a.positions[t] = p;
+  }
+}
+
+// One workgroup: requests that end are few.
+__global__ __launch_bounds__(kThreads) void release_kernel(int num, int block, int width, int capacity,
+                                                           const int* __restrict__ finished,
+                                                           const int* __restrict__ table, int* contexts,
+                                                           int* free_blocks, const int* free_count,
+                                                           int* free_left) {
+  __shared__ int scan_lds[kThreads / 64];
+  int count = min(max(free_count[0], 0), capacity);
+  for (int base = 0; base < num; base += kThreads) {
+    const int r = base + threadIdx.x;
+    int blocks = 0;
+    if (r < num && finished[r]) {
+      const long tokens = min(max(contexts[r], 0), kMaxLength);
+      blocks = min(static_cast<int>((tokens + block - 1) / block), min(width, kMaxCount));
+      contexts[r] = 0;
+    }
+    int all;
+    const int at = block_scan(blocks, scan_lds, &all);
+    for (int j = 0; j < blocks && static_cast<long>(count) + at + j < capacity; ++j)
+      free_blocks[count + at + j] = table[static_cast<long>(r) * width + j];
+    count = static_cast<int>(min(static_cast<long>(count) + all, static_cast<long>(capacity)));
+  }
+  if (threadIdx.x == 0) free_left[0] = count;
+}
+
+}  // namespace
+}  // namespace mchip
+
+using namespace mchip;
+
+extern "C" int mcCacheReserve(int num_requests, int block_size, int table_width, int max_tokens,
+                              int free_capacity, const int* cached_lens, const int* new_lens,
+                              const int* free_blocks, const int* free_count, int* block_table,
+                              int* context_lens, int* row_starts, int* slots, int* positions,
+                              int* free_left, int* denied, void* stream) {
+  MC_REQUIRE(num_requests >= 0 && num_requests <= kMaxRequests,
+             "mcCacheReserve: %d requests (0 to %d are possible)", num_requests, kMaxRequests);
+  MC_REQUIRE(block_size > 0 && table_width > 0, "mcCacheReserve: bad block size or table width");
+  MC_REQUIRE(max_tokens >= 0 && max_tokens < kMaxCount && free_capacity >= 0 && free_capacity < kMaxCount,
+             "mcCacheReserve: %d tokens, %d free blocks (0 to %d are possible)", max_tokens,
+             free_capacity, kMaxCount - 1);
+  MC_REQUIRE(num_requests == 0 || (cached_lens && new_lens && block_table && context_lens),
+             "mcCacheReserve: null argument");
+  MC_REQUIRE(free_count && row_starts && free_left && denied && (free_blocks || !free_capacity) &&
+                 ((slots && positions) || !max_tokens),
+             "mcCacheReserve: null argument");
+  MC_REQUIRE(free_count != free_left, "mcCacheReserve: free_left must not be free_count");
+  MC_REQUIRE(cached_lens != context_lens || num_requests == 0,
+             "mcCacheReserve: context_lens must not be cached_lens");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const ReserveArgs a = {num_requests, block_size, table_width, max_tokens, free_capacity, cached_lens,
+                         new_lens, free_blocks, free_count, block_table, context_lens, row_starts, slots,
+                         positions, free_left, denied};
+  const int blocks = std::min(std::max(ceil_div(max_tokens, kThreads), 1), kNumCu);
+  reserve_kernel<<<blocks, kThreads, 2 * sizeof(int) * num_requests, st>>>(a);
+  MC_LAUNCH_CHECK();
+  return 0;
+}
+
+extern "C" int mcCacheRelease(int num_requests, int block_size, int table_width, int free_capacity,
+                              const int* finished, const int* block_table, int* context_lens,
+                              int* free_blocks, const int* free_count, int* free_left, void* stream) {
+  MC_REQUIRE(num_requests >= 0 && block_size > 0 && table_width > 0 && free_capacity >= 0 &&
+                 free_capacity < kMaxCount,
+             "mcCacheRelease: bad extents");
+  MC_REQUIRE(num_requests == 0 || (finished && block_table && context_lens),
+             "mcCacheRelease: null argument");
+  MC_REQUIRE(free_count && free_left && (free_blocks || !free_capacity), "mcCacheRelease: null argument");
+  release_kernel<<<1, kThreads, 0, static_cast<hipStream_t>(stream)>>>(
+      num_requests, block_size, table_width, free_capacity, finished, block_table, context_lens,
+      free_blocks, free_count, free_left);
+  MC_LAUNCH_CHECK();
+  return 0;
+}

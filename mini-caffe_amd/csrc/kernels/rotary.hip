@@ -1,0 +1,212 @@
+// Rotary positions with several axes, and the store of keys and values into a paged cache.
+//
+// Pair i of a head is a complex number, turned by angle = position[axis(i)] * frequency[i]
+// (rounded to 32 bits): (a, b) -> (a cos - b sin, b cos + a sin).  All heads of a token turn
+// by the same angles, so a workgroup forms a token's cosines and sines once, in LDS, and
+// then passes over its query, key and value heads.  Every value is read and written once:
+// the bound is HBM.
+#include "rows_of_heads.h"
+
+#include <algorithm>
+
+namespace mchip {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxPairs = kMaxHeadDim / 2;
+
+struct RotaryArgs {
+  int heads, heads_kv, head_dim, pairs, tokens;
+  const float* frequencies;
+  const int* positions;
+  long axis_stride;
+  mcHeads q, q_out, k, k_out, v;  // data null: not there
+  mcPagedCache cache;             // keys null: none
+  const int* slots;
+  unsigned char axis[kMaxPairs];
+};
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load(const T* p) {
+  return *reinterpret_cast<const Pack<T, N>*>(p);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store(T* p, const Pack<T, N>& x) {
+  *reinterpret_cast<Pack<T, N>*>(p) = x;
+}
+
+__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
+  const float x = a * c - b * s;
+  b = b * c + a * s;
+  a = x;
+}
+
+// One head's chunk c of a row: N pairs turned, or N values copied.  rotated chunks come first.
+template <typename T, int N, bool ADJACENT>
+__device__ __forceinline__ void head_chunk(const T* src, T* dst, T* dst2, int c, int rotated, int pairs,
+                                           const float* cs, const float* sn) {
+  if (c < rotated) {
+    const int i = c * N;  // first pair
+    float co[N], si[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) co[e] = cs[i + e], si[e] = sn[i + e];
+    const int o0 = ADJACENT ? 2 * i : i, o1 = ADJACENT ? 2 * i + N : pairs + i;
+    Pack<T, N> x = load<T, N>(src + o0), y = load<T, N>(src + o1);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      // neighbours: pair e lies in x (first half of the 2N values) or y
+      T& ta = ADJACENT ? (2 * e < N ? x.v[(2 * e) % N] : y.v[(2 * e) % N]) : x.v[e];
+      T& tb = ADJACENT ? (2 * e + 1 < N ? x.v[(2 * e + 1) % N] : y.v[(2 * e + 1) % N]) : y.v[e];
+      float a = static_cast<float>(ta), b = static_cast<float>(tb);
+      turn(a, b, co[e], si[e]);
+      ta = static_cast<T>(a);
+      tb = static_cast<T>(b);
+    }
+    if (dst) store<T, N>(dst + o0, x), store<T, N>(dst + o1, y);
+    if (dst2) store<T, N>(dst2 + o0, x), store<T, N>(dst2 + o1, y);
+  } else {
+    const int o = 2 * pairs + (c - rotated) * N;
+    const Pack<T, N> x = load<T, N>(src + o);
+    if (dst) store<T, N>(dst + o, x);
+    if (dst2) store<T, N>(dst2 + o, x);
+  }
+}
+
+// A workgroup per token.  N: pairs of a chunk, a divisor of `pairs`.
+template <typename T, int N, bool ADJACENT>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
+  __shared__ float cs[kMaxPairs], sn[kMaxPairs];
+  const int t = blockIdx.x, tid = threadIdx.x;
+  if (tid < a.pairs)
+    sincosf(static_cast<float>(a.positions[a.axis[tid] * a.axis_stride + t]) * a.frequencies[tid], &sn[tid],
+            &cs[tid]);
+  __syncthreads();
+  long cache_row = -1;
+  if (a.cache.keys) {
+    const int s = a.slots[t];
+    if (s >= 0 && s < a.cache.num_blocks * a.cache.block_size)
+      cache_row = (s / a.cache.block_size) * a.cache.block_stride + (s % a.cache.block_size) * a.cache.token_stride;
+  }
+  const int rotated = a.pairs / N, chunks = rotated + (a.head_dim - 2 * a.pairs) / N;
+  for (int i = tid; i < chunks * a.heads; i += kThreads) {
+    const int h = i / chunks, c = i - h * chunks;
+    head_chunk<T, N, ADJACENT>(static_cast<const T*>(a.q.data) + t * a.q.token_stride + h * a.q.head_stride,
+                               static_cast<T*>(a.q_out.data) + t * a.q_out.token_stride + h * a.q_out.head_stride,
+                               nullptr, c, rotated, a.pairs, cs, sn);
+  }
+  if (a.k.data)
+    for (int i = tid; i < chunks * a.heads_kv; i += kThreads) {
+      const int h = i / chunks, c = i - h * chunks;
+      T* out = a.k_out.data ? static_cast<T*>(a.k_out.data) + t * a.k_out.token_stride + h * a.k_out.head_stride
+                            : nullptr;
+      T* kept = cache_row >= 0 ? static_cast<T*>(a.cache.keys) + cache_row + h * a.cache.head_stride : nullptr;
+      head_chunk<T, N, ADJACENT>(static_cast<const T*>(a.k.data) + t * a.k.token_stride + h * a.k.head_stride,
+                                 out, kept, c, rotated, a.pairs, cs, sn);
+    }
+  if (a.v.data && cache_row >= 0) {
+    constexpr int V = 16 / sizeof(T);
+    const int vc = a.head_dim / V;
+    for (int i = tid; i < vc * a.heads_kv; i += kThreads) {
+      const int h = i / vc, c = i - h * vc;
+      store<T, V>(static_cast<T*>(a.cache.values) + cache_row + h * a.cache.head_stride + c * V,
+                  load<T, V>(static_cast<const T*>(a.v.data) + t * a.v.token_stride + h * a.v.head_stride + c * V));
+    }
+  }
+}
+
+template <typename T, int N>
+void launch(const RotaryArgs& a, bool adjacent, hipStream_t st) {
+  if (adjacent) rotary_kernel<T, N, true><<<a.tokens, kThreads, 0, st>>>(a);
+  else rotary_kernel<T, N, false><<<a.tokens, kThreads, 0, st>>>(a);
+}
+
+// The widest chunk, up to 16 bytes, that divides both halves of the turned part.
+template <typename T>
+void launch_chunk(const RotaryArgs& a, bool adjacent, hipStream_t st) {
+  if (sizeof(T) == 2 && a.pairs % 8 == 0) launch<T, 16 / sizeof(T)>(a, adjacent, st);
+  else if (a.pairs % 4 == 0) launch<T, 4>(a, adjacent, st);
+  else if (a.pairs % 2 == 0) launch<T, 2>(a, adjacent, st);
+  else launch<T, 1>(a, adjacent, st);
+}
+
+}  // namespace
+}  // namespace mchip
+
+using namespace mchip;
+
+extern "C" int mcRotary(const mcRotaryGeom* geom, const float* frequencies, const int* positions,
+                        long axis_stride, int tokens, const mcHeads* q, const mcHeads* q_out,
+                        const mcHeads* k, const mcHeads* k_out, const mcHeads* v,
+                        const mcPagedCache* cache, const int* slots, void* stream) {
+  static const char who[] = "mcRotary";
+  MC_REQUIRE(geom, "%s: null geometry", who);
+  if (check_type(who, geom->type, geom->head_dim)) return -1;
+  MC_REQUIRE(geom->heads > 0 && geom->heads_kv >= 0, "%s: %d query heads, %d key heads", who, geom->heads,
+             geom->heads_kv);
+  MC_REQUIRE(geom->rotary_dim > 0 && geom->rotary_dim % 2 == 0 && geom->rotary_dim <= geom->head_dim,
+             "%s: rotary_dim %d is not even or not in 2 .. head_dim %d", who, geom->rotary_dim, geom->head_dim);
+  MC_REQUIRE(geom->num_axes >= 1 && geom->num_axes <= 4, "%s: %d axes (1 to 4 are possible)", who,
+             geom->num_axes);
+  RotaryArgs a = {};
+  a.pairs = geom->rotary_dim / 2;
+  int left[4] = {0, 0, 0, 0}, sum = 0;
+  for (int i = 0; i < geom->num_axes; ++i) {
+    MC_REQUIRE(geom->sections[i] >= 0 && geom->sections[i] <= a.pairs, "%s: section %d is %d", who, i,
+               geom->sections[i]);
+    sum += left[i] = geom->sections[i];
+  }
+  MC_REQUIRE(sum == a.pairs, "%s: the sections hold %d pairs of %d", who, sum, a.pairs);
+  for (int i = 0, axis = 0; i < a.pairs; ++i) {
+    while (left[axis] == 0) axis = (axis + 1) % geom->num_axes;
+    a.axis[i] = static_cast<unsigned char>(axis);
+    --left[axis];
+    if (geom->cycled) axis = (axis + 1) % geom->num_axes;
+  }
+  MC_REQUIRE(tokens >= 0, "%s: %d tokens", who, tokens);
+  if (tokens == 0) return 0;
+  MC_REQUIRE(frequencies && positions, "%s: null argument", who);
+  if (check_heads(who, "q", q, geom->type) || check_heads(who, "q_out", q_out, geom->type)) return -1;
+  a.q = *q;
+  a.q_out = *q_out;
+  MC_REQUIRE(geom->heads_kv > 0 || !(k || v), "%s: keys or values without heads_kv", who);
+  MC_REQUIRE(k || !k_out, "%s: k_out without k", who);
+  MC_REQUIRE(cache || !v, "%s: values without a cache", who);
+  if (k) {
+    if (check_heads(who, "k", k, geom->type)) return -1;
+    a.k = *k;
+    MC_REQUIRE(k_out || cache, "%s: keys with neither k_out nor a cache", who);
+    if (k_out) {
+      if (check_heads(who, "k_out", k_out, geom->type)) return -1;
+      a.k_out = *k_out;
+    }
+  }
+  if (v) {
+    if (check_heads(who, "v", v, geom->type)) return -1;
+    a.v = *v;
+  }
+  if (cache) {
+    if (check_cache(who, cache, geom->type)) return -1;
+    MC_REQUIRE(slots, "%s: a cache without slots", who);
+    a.cache = *cache;
+  }
+  a.slots = slots;
+  a.heads = geom->heads;
+  a.heads_kv = geom->heads_kv;
+  a.head_dim = geom->head_dim;
+  a.tokens = tokens;
+  a.frequencies = frequencies;
+  a.positions = positions;
+  a.axis_stride = axis_stride;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool adjacent = geom->adjacent != 0;
+  if (geom->type == MC_TYPE_F32) launch_chunk<float>(a, adjacent, st);
+  else if (geom->type == MC_TYPE_F16) launch_chunk<half_t>(a, adjacent, st);
+  else launch_chunk<bf16_t>(a, adjacent, st);
+  MC_LAUNCH_CHECK();
+  return 0;
+}

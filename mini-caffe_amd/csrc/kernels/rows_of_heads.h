@@ -1,0 +1,55 @@
+// Element types and addressing that the operators of language models share: rows of heads
+// and a paged cache (mcHeads, mcPagedCache), checked on the host and passed by value.
+#ifndef MCHIP_ROWS_OF_HEADS_H_
+#define MCHIP_ROWS_OF_HEADS_H_
+
+#include "mc_common.h"
+#include "mchip/kernels.h"
+
+#include <climits>
+#include <cstdint>
+
+namespace mchip {
+
+using half_t = _Float16;
+using bf16_t = __bf16;
+
+constexpr int kMaxHeadDim = 256;
+
+inline size_t type_size(int type) { return type == MC_TYPE_F32 ? 4 : 2; }
+
+// The 16-byte rule: every row of every head then starts where 16-byte loads may.
+inline bool rows_aligned(const void* data, size_t size, long a, long b, long c = 0) {
+  const long per = static_cast<long>(16 / size);
+  return (reinterpret_cast<uintptr_t>(data) & 15) == 0 && a % per == 0 && b % per == 0 && c % per == 0;
+}
+
+inline int check_heads(const char* who, const char* what, const mcHeads* h, int type) {
+  MC_REQUIRE(h && h->data, "%s: %s is null", who, what);
+  MC_REQUIRE(rows_aligned(h->data, type_size(type), h->token_stride, h->head_stride),
+             "%s: %s: data and strides are not multiples of 16 bytes", who, what);
+  return 0;
+}
+
+inline int check_cache(const char* who, const mcPagedCache* c, int type) {
+  MC_REQUIRE(c && c->keys && c->values, "%s: the cache is null", who);
+  MC_REQUIRE(c->num_blocks > 0 && c->block_size > 0, "%s: the cache has no blocks", who);
+  MC_REQUIRE(static_cast<long>(c->num_blocks) * c->block_size <= INT_MAX,
+             "%s: more than 2^31 - 1 slots in the cache", who);
+  MC_REQUIRE(rows_aligned(c->keys, type_size(type), c->block_stride, c->token_stride, c->head_stride) &&
+                 rows_aligned(c->values, type_size(type), 0, 0),
+             "%s: the cache's data and strides are not multiples of 16 bytes", who);
+  return 0;
+}
+
+inline int check_type(const char* who, int type, int head_dim) {
+  MC_REQUIRE(type == MC_TYPE_F32 || type == MC_TYPE_F16 || type == MC_TYPE_BF16,
+             "%s: unknown element type %d", who, type);
+  MC_REQUIRE(head_dim >= 8 && head_dim <= kMaxHeadDim && head_dim % 8 == 0,
+             "%s: head_dim %d is not a multiple of 8 in 8 .. %d", who, head_dim, kMaxHeadDim);
+  return 0;
+}
+
+}  // namespace mchip
+
+#endif  // MCHIP_ROWS_OF_HEADS_H_

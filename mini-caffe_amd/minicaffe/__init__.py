@@ -7,6 +7,7 @@ from .base import LIB, LIB_PATH, MiniCaffeError, check_call  # noqa: F401
 from .blob import Blob  # noqa: F401
 from .net import Net  # noqa: F401
 from . import kernels  # noqa: F401  (declares the prototypes of the mc* kernel entry points)
+from . import attention  # noqa: F401
 
 
 def check_gpu_available():

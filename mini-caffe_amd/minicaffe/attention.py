@@ -1,0 +1,104 @@
+"""Attention of language models over image and text tokens: ctypes prototypes of the
+entry points in include/mchip/kernels.h, next to those of minicaffe.kernels.
+
+As there, arrays are raw device addresses (ints) that the caller owns, `stream` is a HIP
+stream handle (0: the null stream), and a failed call raises with the library's message.
+`heads_of` and `PagedCache.of` describe torch tensors.
+"""
+import ctypes
+
+from .base import LIB, check_mc
+
+c_void_p, c_int, c_long, c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
+
+F32, F16, BF16 = 0, 1, 2
+TYPES = {"f32": F32, "f16": F16, "bf16": BF16}
+
+
+class Heads(ctypes.Structure):
+    """Rows of heads: head h of token t at element t * token_stride + h * head_stride."""
+    _fields_ = [("data", c_void_p), ("token_stride", c_long), ("head_stride", c_long)]
+
+
+class PagedCache(ctypes.Structure):
+    """Keys and values in blocks of block_size slots; see mcPagedCache."""
+    _fields_ = [("keys", c_void_p), ("values", c_void_p), ("num_blocks", c_int), ("block_size", c_int),
+                ("block_stride", c_long), ("token_stride", c_long), ("head_stride", c_long)]
+
+    @classmethod
+    def of(cls, keys, values):
+        """Of tensors [blocks, block_size, heads_kv, head_dim]."""
+        _check_rows(keys)
+        _check_rows(values)
+        if keys.shape != values.shape or keys.stride() != values.stride():
+            raise ValueError("keys and values of a cache have one shape and one layout")
+        return cls(keys.data_ptr(), values.data_ptr(), keys.shape[0], keys.shape[1], *keys.stride()[:3])
+
+
+class RotaryGeom(ctypes.Structure):
+    _fields_ = [("type", c_int), ("heads", c_int), ("heads_kv", c_int), ("head_dim", c_int), ("rotary_dim", c_int),
+                ("adjacent", c_int), ("num_axes", c_int), ("sections", c_int * 4), ("cycled", c_int)]
+
+
+class AttentionGeom(ctypes.Structure):
+    _fields_ = [("type", c_int), ("heads", c_int), ("heads_kv", c_int), ("head_dim", c_int), ("causal", c_int),
+                ("scale", c_float)]
+
+
+_heads_p, _cache_p = ctypes.POINTER(Heads), ctypes.POINTER(PagedCache)
+LIB.mcCacheReserve.argtypes = [c_int] * 5 + [c_void_p] * 12
+LIB.mcCacheRelease.argtypes = [c_int] * 4 + [c_void_p] * 7
+LIB.mcRotary.argtypes = [ctypes.POINTER(RotaryGeom), c_void_p, c_void_p, c_long, c_int] + [_heads_p] * 5 + \
+    [_cache_p, c_void_p, c_void_p]
+LIB.mcAttentionPacked.argtypes = [ctypes.POINTER(AttentionGeom)] + [_heads_p] * 3 + [c_void_p] * 2 + [c_int] * 3 + \
+    [_heads_p, c_void_p, c_void_p]
+LIB.mcAttentionPaged.argtypes = [ctypes.POINTER(AttentionGeom), _heads_p, _cache_p, c_void_p, c_int, c_void_p, c_void_p] + \
+    [c_int] * 4 + [_heads_p, c_void_p, c_void_p]
+
+
+def _check_rows(tensor):
+    if tensor.stride(-1) != 1:
+        raise ValueError("the values of a head have to be contiguous")
+
+
+def heads_of(tensor):
+    """Of a tensor [tokens, heads, head_dim], a slice or a transposed view among them."""
+    if tensor.dim() != 3:
+        raise ValueError("heads_of: a tensor [tokens, heads, head_dim] is wanted")
+    _check_rows(tensor)
+    return Heads(tensor.data_ptr(), tensor.stride(0), tensor.stride(1))
+
+
+def rotary_geom(type, heads, heads_kv, head_dim, rotary_dim, sections, adjacent=False, cycled=False):
+    if not 1 <= len(sections) <= 4:
+        raise ValueError("rotary_geom: one to four axes")
+    return RotaryGeom(type, heads, heads_kv, head_dim, rotary_dim, int(adjacent), len(sections),
+                      (c_int * 4)(*sections), int(cycled))
+
+
+def cache_reserve(num_requests, block_size, table_width, max_tokens, free_capacity, cached_lens, new_lens, free_blocks,
+                  free_count, block_table, context_lens, row_starts, slots, positions, free_left, denied, stream=0):
+    check_mc(LIB.mcCacheReserve(num_requests, block_size, table_width, max_tokens, free_capacity, cached_lens, new_lens,
+                                free_blocks, free_count, block_table, context_lens, row_starts, slots, positions, free_left,
+                                denied, stream))
+
+
+def cache_release(num_requests, block_size, table_width, free_capacity, finished, block_table, context_lens, free_blocks,
+                  free_count, free_left, stream=0):
+    check_mc(LIB.mcCacheRelease(num_requests, block_size, table_width, free_capacity, finished, block_table, context_lens,
+                                free_blocks, free_count, free_left, stream))
+
+
+def rotary(geom, frequencies, positions, axis_stride, tokens, q, q_out, k=None, k_out=None, v=None, cache=None, slots=None,
+           stream=0):
+    check_mc(LIB.mcRotary(geom, frequencies, positions, axis_stride, tokens, q, q_out, k, k_out, v, cache, slots, stream))
+
+
+def attention_packed(geom, q, k, v, q_starts, k_starts, num_sequences, total_q, total_k, out, lse=None, stream=0):
+    check_mc(LIB.mcAttentionPacked(geom, q, k, v, q_starts, k_starts, num_sequences, total_q, total_k, out, lse, stream))
+
+
+def attention_paged(geom, q, cache, block_table, table_width, q_starts, context_lens, num_requests, total_q, max_q,
+                    max_context, out, lse=None, stream=0):
+    check_mc(LIB.mcAttentionPaged(geom, q, cache, block_table, table_width, q_starts, context_lens, num_requests, total_q,
+                                  max_q, max_context, out, lse, stream))
