@@ -1,0 +1,97 @@
+// Launches of the attention kernels for one element type; each type is a source file of its
+// own, which keeps the build short.
+#ifndef MCHIP_ATTENTION_LAUNCH_H_
+#define MCHIP_ATTENTION_LAUNCH_H_
+
+#include "attention_tile.h"
+
+#include <algorithm>
+
+namespace mchip {
+namespace {
+
+// Rows whose keys were cut into pieces: the pieces' sums, weighted by e^(m_piece - m).  One
+// wavefront per row and head.
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs a) {
+  const long at = blockIdx.x * 4l + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (at >= static_cast<long>(a.total_q) * a.heads) return;
+  const int token = static_cast<int>(at / a.heads), head = static_cast<int>(at - static_cast<long>(token) * a.heads);
+  const int seq = sequence_of_tile(a.q_starts, a.num, 1, 1, token, 0);
+  const int q0 = max(a.q_starts[seq], 0), q1 = min(a.q_starts[seq + 1], a.total_q);
+  const int queries = min(q1 - q0, a.max_q);
+  if (token < q0 || token - q0 >= queries) return;
+  const int all = keys_of_tile<true>(a, keys_of<true>(a, seq, q1 - q0), (token - q0) * static_cast<int>(a.group.d) +
+                                     head % static_cast<int>(a.group.d), queries * static_cast<int>(a.group.d));
+  if (all <= a.piece) return;  // written by the one workgroup that had all of its keys
+  const int pieces = (all + a.piece - 1) / a.piece;
+  const long step = static_cast<long>(a.total_q) * a.heads;
+  float m = -INFINITY;
+  for (int p = 0; p < pieces; ++p) m = fmaxf(m, a.stats[2 * (p * step + at)]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[(DP + 63) / 64] = {};
+  for (int p = 0; p < pieces; ++p) {
+    const long from = p * step + at;
+    const float w = exp2f(a.stats[2 * from] - base);
+    l += w * a.stats[2 * from + 1];
+#pragma unroll
+    for (int i = 0; i < (DP + 63) / 64; ++i)
+      if (lane + 64 * i < DP) o[i] += w * a.partial[from * DP + lane + 64 * i];
+  }
+  const float inverse = l == 0.f ? 0.f : 1.f / l;
+  T* out = static_cast<T*>(a.out.data) + token * a.out.token_stride + head * a.out.head_stride;
+#pragma unroll
+  for (int i = 0; i < (DP + 63) / 64; ++i)
+    if (lane + 64 * i < a.head_dim) out[lane + 64 * i] = static_cast<T>(o[i] * inverse);
+  if (a.lse && lane == 0)
+    a.lse[static_cast<long>(head) * a.total_q + token] =
+        l == 0.f ? -INFINITY : (m - kLift<T> + log2f(l)) * 0.69314718f;
+}
+
+template <typename T, int DP, bool PAGED>
+int launch_tiles(AttentionArgs a, hipStream_t st) {
+  constexpr int kKeys = TileShape<T, DP>::kKeys;
+  const long group = a.group.d;
+  a.tiles = static_cast<int>(a.total_q * group / kTileRows) + a.num;
+  a.pieces = 1;
+  a.piece = a.max_context;
+  if (PAGED) {
+    // too few tiles to fill the GPU: cut the keys, in pieces of at least four tiles of keys
+    const long items = static_cast<long>(a.tiles) * a.heads_kv;
+    const int most = std::max(1, a.max_context / (4 * kKeys));
+    const int wanted = static_cast<int>(std::min<long>(std::max<long>(1, 2 * kNumCu / items), most));
+    a.piece = std::max(ceil_div(ceil_div(a.max_context, wanted), kKeys), 1) * kKeys;
+    a.pieces = std::max(1, ceil_div(a.max_context, a.piece));
+    if (a.pieces > 1) {
+      const long rows = static_cast<long>(a.total_q) * a.heads * a.pieces;
+      float* scratch;
+      if (stream_workspace(st, static_cast<size_t>(rows) * (DP + 2) * sizeof(float), &scratch)) return -1;
+      a.partial = scratch;
+      a.stats = scratch + rows * DP;
+    }
+  }
+  const long blocks = static_cast<long>(a.tiles) * a.heads_kv * a.pieces;
+  MC_REQUIRE(blocks <= INT_MAX, "attention: %ld workgroups", blocks);
+  attention_tile_kernel<T, DP, PAGED><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+  MC_LAUNCH_CHECK();
+  if (PAGED && a.pieces > 1) {
+    attention_join_kernel<T, DP><<<ceil_div(static_cast<long>(a.total_q) * a.heads, 4), 256, 0, st>>>(a);
+    MC_LAUNCH_CHECK();
+  }
+  return 0;
+}
+
+template <typename T, bool PAGED>
+int launch_type(const AttentionArgs& a, hipStream_t st) {
+  if (a.head_dim <= 64) return launch_tiles<T, 64, PAGED>(a, st);
+  if (a.head_dim <= 96) return launch_tiles<T, 96, PAGED>(a, st);
+  if (a.head_dim <= 128) return launch_tiles<T, 128, PAGED>(a, st);
+  if (a.head_dim <= 192) return launch_tiles<T, 192, PAGED>(a, st);
+  return launch_tiles<T, 256, PAGED>(a, st);
+}
+
+}  // namespace
+}  // namespace mchip
+
+#endif  // MCHIP_ATTENTION_LAUNCH_H_
