@@ -47,7 +47,10 @@ extern "C" int mcAttentionPacked(const mcAttentionGeom* geom, const mcHeads* q, 
   MC_REQUIRE(q_starts && k_starts, "%s: null argument", who);
   if (check_heads(who, "q", q, geom->type) || check_heads(who, "out", out, geom->type)) return -1;
   if (total_k > 0) {
-    if (check_heads(who, "k", k, geom->type) || check_heads(who, "v", v, geom->type)) return -1;
+    if (check_heads(who, "k", k, geom->type) || check_heads(who, "v", v, geom->type) ||
+        check_key_stride(who, "k", k->token_stride, geom->type) ||
+        check_key_stride(who, "v", v->token_stride, geom->type))
+      return -1;
     a.k = *k;
     a.v = *v;
   }
@@ -75,7 +78,8 @@ extern "C" int mcAttentionPaged(const mcAttentionGeom* geom, const mcHeads* q, c
   if (num_requests == 0 || total_q == 0 || max_q == 0) return 0;
   MC_REQUIRE(block_table && q_starts && context_lens, "%s: null argument", who);
   if (check_heads(who, "q", q, geom->type) || check_heads(who, "out", out, geom->type) ||
-      check_cache(who, cache, geom->type))
+      check_cache(who, cache, geom->type) ||
+      check_key_stride(who, "cache", cache->token_stride, geom->type))
     return -1;
   a.q = *q;
   a.out = *out;

@@ -73,7 +73,12 @@ int launch_tiles(AttentionArgs a, hipStream_t st) {
   }
   const long blocks = static_cast<long>(a.tiles) * a.heads_kv * a.pieces;
   MC_REQUIRE(blocks <= INT_MAX, "attention: %ld workgroups", blocks);
-  attention_tile_kernel<T, DP, PAGED><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+  if (!PAGED)
+    attention_tile_kernel<T, DP, Source::kPacked><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+  else if (a.cache.block_size % TileShape<T, DP>::kPass == 0)
+    attention_tile_kernel<T, DP, Source::kRuns><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+  else
+    attention_tile_kernel<T, DP, Source::kPaged><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
   MC_LAUNCH_CHECK();
   if (PAGED && a.pieces > 1) {
     attention_join_kernel<T, DP><<<ceil_div(static_cast<long>(a.total_q) * a.heads, 4), 256, 0, st>>>(a);

@@ -20,6 +20,8 @@
 
 #include "attention_args.h"
 
+#include <type_traits>
+
 namespace mchip {
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -49,8 +51,18 @@ struct TileShape {
   // apart) row pieces of a read lie side by side modulo 256 bytes.
   static constexpr int kKStride = (kChunks | 1) * 16;
   static constexpr int kVStride = sizeof(T) == 2 ? ((kRowBytes / 32) | 1) * 32 : kRowBytes + 32;
-  static constexpr int kStage = kKeys * kChunks / 256;         // 16-byte loads per thread, of K and of V
-  static_assert(kKeys * kChunks % 256 == 0, "the tile does not fill the threads evenly");
+  // Staging: a thread carries one chunk (of a power of two, the last ones idle) of kStage rows.
+  static constexpr int kLanes = kChunks <= 8 ? 8 : kChunks <= 16 ? 16 : kChunks <= 32 ? 32 : 64;
+  static constexpr int kPass = 256 / kLanes;                   // rows that the workgroup loads at once
+  static constexpr int kStage = kKeys / kPass;
+};
+
+// Where the keys are.
+enum class Source {
+  kPacked,  // rows of one tensor
+  kRuns,    // a paged cache whose block size is a multiple of kPass: the rows loaded at once
+            // lie in one block, so addresses are scalars plus a fixed offset per thread
+  kPaged    // any block size: a lane looks a key up
 };
 
 // Scores of 32 keys (rows `base` on of the K tile) against the wavefront's rows.
@@ -148,6 +160,15 @@ __device__ __forceinline__ void add_not_finite(const char* lds_v, int seen, unsi
   }
 }
 
+// The larger of the lane's value and that of lane ^ 32.  (The two results of the builtin
+// for this instruction are taken as equal when its operands are, so it is written out; a
+// vector result needs two wait states before a lane exchange reads it.)
+__device__ __forceinline__ float larger_of_halves(float x) {
+  float y = x;
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));  // {low, low}, {high, high}
+  return fmaxf(x, y);
+}
+
 // The running softmax of one row: powers of two of the scores times scale * log2(e).  The
 // sum is the lane's own half of the keys until the end.
 struct Running {
@@ -173,7 +194,7 @@ __device__ __forceinline__ void softmax_step(floatx16* s, floatx16* o, Running& 
   for (int u = 0; u < SUB; ++u)
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
-  top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale_log2;
+  top = larger_of_halves(top) * scale_log2;
   if (__any(top > r.m + kSlack<T>)) {
     const float m = fmaxf(r.m, top);
     const float keep = m == -INFINITY ? 1.f : exp2f(r.m - m);
@@ -231,15 +252,16 @@ __device__ __forceinline__ void store_rows(const AttentionArgs& a, const floatx1
         r.l == 0.f ? -INFINITY : (r.m - kLift<T> + log2f(r.l)) * 0.69314718f;
 }
 
-template <typename T, int DP, bool PAGED>
+template <typename T, int DP, Source SRC>
 __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_tile_kernel(
     const AttentionArgs a) {
   using S = TileShape<T, DP>;
+  constexpr bool PAGED = SRC != Source::kPacked;
   constexpr int KT = S::kKeys, SUB = KT / 32;
   __shared__ __attribute__((aligned(16))) char lds_k[2][KT * S::kKStride];
   __shared__ __attribute__((aligned(16))) char lds_v[2][KT * S::kVStride];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = a.group.d, D = a.head_dim;
   // key heads vary fastest: with workgroups dealt to the XCDs in turn, eight key heads (or
   // a divisor or multiple of eight) put each one's keys into one XCD's L2.  Tiles run from
@@ -260,12 +282,9 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_
   const bool real = first + 32 * wave + (lane & 31) < rows;
   const int token = a.group.quotient(row), head = hk * group + (row - token * group);
   const int limit = max(min(keys.count, a.causal ? keys.offset + token : keys.count), 0);
-  int low = limit, high = limit;  // over the wavefront's rows
-#pragma unroll
-  for (int w = 16; w > 0; w >>= 1) {
-    low = min(low, __shfl_xor(low, w, 64));
-    high = max(high, __shfl_xor(high, w, 64));
-  }
+  // rows see more from the first to the last of a wavefront
+  const int low = __builtin_amdgcn_readfirstlane(limit);
+  const int high = __builtin_amdgcn_readlane(limit, 31);
   const int all = keys_of_tile<PAGED>(a, keys, first, rows);  // over the workgroup's
   const int begin = PAGED ? min(piece * a.piece, all) : 0;
   const int end = PAGED ? static_cast<int>(min(static_cast<long>(begin) + a.piece, static_cast<long>(all))) : all;
@@ -284,115 +303,164 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_
     }
   }
 
-  // staging: thread t carries chunk t % kChunks (rounded over the loads) of some rows
-  const T* kbase = static_cast<const T*>(PAGED ? a.cache.keys : a.k.data) +
-                   hk * (PAGED ? a.cache.head_stride : a.k.head_stride);
-  const T* vbase = static_cast<const T*>(PAGED ? a.cache.values : a.v.data) +
-                   hk * (PAGED ? a.cache.head_stride : a.v.head_stride);
+  // Staging.  Chunks past head_dim are zeroed in LDS once and not written again.
+  const int chunk = tid % S::kLanes, pass_row = tid / S::kLanes;
+  const bool there = chunk * static_cast<int>(16 / sizeof(T)) < D;
+  const long k_stride = (PAGED ? a.cache.token_stride : a.k.token_stride) * static_cast<long>(sizeof(T));
+  const long v_stride = (PAGED ? a.cache.token_stride : a.v.token_stride) * static_cast<long>(sizeof(T));
+  const char* kbase = reinterpret_cast<const char*>(
+      static_cast<const T*>(PAGED ? a.cache.keys : a.k.data) +
+      hk * (PAGED ? a.cache.head_stride : a.k.head_stride) + (PAGED ? 0 : keys.first * a.k.token_stride));
+  const char* vbase = reinterpret_cast<const char*>(
+      static_cast<const T*>(PAGED ? a.cache.values : a.v.data) +
+      hk * (PAGED ? a.cache.head_stride : a.v.head_stride) + (PAGED ? 0 : keys.first * a.v.token_stride));
+  const unsigned chunk_at = there ? chunk * 16 : 0;
+  const unsigned k_off = pass_row * static_cast<unsigned>(k_stride) + chunk_at;
+  const unsigned v_off = pass_row * static_cast<unsigned>(v_stride) + chunk_at;
   const int* table = PAGED ? a.block_table + static_cast<long>(seq) * a.table_width : nullptr;
-  floatx4 stage_k[S::kStage], stage_v[S::kStage];
-  unsigned long stage_valid = ~0ul;
-  auto fetch = [&](int tile_begin) {  // keys past the end repeat the last one
-    long at = 0;
-    if (PAGED) {
-      const int key = tile_begin + (lane % KT);
-      at = cache_row(a, table, min(key, end - 1));
-      stage_valid = __ballot(at >= 0 && key < end);
-      at = max(at, 0l);
-    }
+  char* const put_k = lds_k[0] + pass_row * S::kKStride + chunk * 16;
+  char* const put_v = lds_v[0] + pass_row * S::kVStride + chunk * 16;
+  if (S::kLanes != S::kChunks || DP != D) {
+    if (!there && chunk < S::kChunks)
 #pragma unroll
-    for (int i = 0; i < S::kStage; ++i) {
-      const int c = tid + 256 * i, r = c / S::kChunks, chunk = c % S::kChunks;
-      const bool there = chunk * static_cast<int>(16 / sizeof(T)) < D;
-      long kat, vat;
-      if (PAGED) {
-        kat = vat = __shfl(at, r, 64);
-      } else {
-        const long key = keys.first + min(tile_begin + r, end - 1);
-        kat = key * a.k.token_stride;
-        vat = key * a.v.token_stride;
+      for (int i = 0; i < 2 * S::kStage; ++i) {
+        const int b = i / S::kStage, r = i % S::kStage * S::kPass;
+        *reinterpret_cast<floatx4*>(put_k + b * KT * S::kKStride + r * S::kKStride) = floatx4{};
+        *reinterpret_cast<floatx4*>(put_v + b * KT * S::kVStride + r * S::kVStride) = floatx4{};
       }
-      stage_k[i] = stage_v[i] = floatx4{};
-      if (there) {
-        stage_k[i] = *reinterpret_cast<const floatx4*>(reinterpret_cast<const char*>(kbase + kat) + chunk * 16);
-        stage_v[i] = *reinterpret_cast<const floatx4*>(reinterpret_cast<const char*>(vbase + vat) + chunk * 16);
+  }
+  floatx4 stage_k[S::kStage], stage_v[S::kStage];
+  constexpr unsigned long kAllValid = KT == 64 ? ~0ul : (1ul << KT) - 1;
+  unsigned long stage_valid = kAllValid;
+  int number[S::kStage];  // kRuns: the next tile's blocks
+  auto look_up = [&](int tile_begin) {
+    if constexpr (SRC == Source::kRuns)
+#pragma unroll
+      for (int i = 0; i < S::kStage; ++i)
+        number[i] = table[a.block.quotient(min(tile_begin + i * S::kPass, end - 1))];
+  };
+  auto fetch = [&](int tile_begin) {  // keys past the end repeat the last one
+    if constexpr (SRC == Source::kPacked) {
+      const char* kt = kbase + tile_begin * k_stride;
+      const char* vt = vbase + tile_begin * v_stride;
+      if (tile_begin + KT <= end) {
+#pragma unroll
+        for (int i = 0; i < S::kStage; ++i) {
+          stage_k[i] = *reinterpret_cast<const floatx4*>(kt + i * S::kPass * k_stride + k_off);
+          stage_v[i] = *reinterpret_cast<const floatx4*>(vt + i * S::kPass * v_stride + v_off);
+        }
+      } else {
+        const int last = end - 1 - tile_begin;
+#pragma unroll
+        for (int i = 0; i < S::kStage; ++i) {
+          const unsigned r = min(pass_row + i * S::kPass, last);
+          stage_k[i] = *reinterpret_cast<const floatx4*>(kt + (r * static_cast<unsigned>(k_stride) + chunk_at));
+          stage_v[i] = *reinterpret_cast<const floatx4*>(vt + (r * static_cast<unsigned>(v_stride) + chunk_at));
+        }
+      }
+    } else if constexpr (SRC == Source::kRuns) {
+      stage_valid = kAllValid;
+#pragma unroll
+      for (int i = 0; i < S::kStage; ++i) {
+        // (rows past the end lie in the last key's block)
+        const unsigned key = min(tile_begin + i * S::kPass, (end - 1) / S::kPass * S::kPass);
+        int n = number[i];
+        if (static_cast<unsigned>(n) >= static_cast<unsigned>(a.cache.num_blocks)) {
+          n = 0;
+          stage_valid &= ~(((1ul << S::kPass) - 1) << (i * S::kPass));
+        }
+        const long at = (n * a.cache.block_stride) * static_cast<long>(sizeof(T)) +
+                        (key - a.block.quotient(key) * a.block.d) * k_stride;
+        unsigned off = k_off;
+        if (tile_begin + KT > end)
+          off = min(pass_row, end - 1 - static_cast<int>(key)) * static_cast<unsigned>(k_stride) + chunk_at;
+        stage_k[i] = *reinterpret_cast<const floatx4*>(kbase + at + off);
+        stage_v[i] = *reinterpret_cast<const floatx4*>(vbase + at + off);
+      }
+      if (tile_begin + KT < end) look_up(tile_begin + KT);
+    } else {
+      const int key = tile_begin + (lane % KT);
+      long at = cache_row(a, table, min(key, end - 1));
+      stage_valid = __ballot(at >= 0 && key < end) & kAllValid;
+      at = max(at, 0l) * static_cast<long>(sizeof(T)) ;
+#pragma unroll
+      for (int i = 0; i < S::kStage; ++i) {
+        const long from = __shfl(at, pass_row + i * S::kPass, 64) + chunk_at;
+        stage_k[i] = *reinterpret_cast<const floatx4*>(kbase + from);
+        stage_v[i] = *reinterpret_cast<const floatx4*>(vbase + from);
       }
     }
   };
   auto put = [&](int buffer) {
+    if (there)
 #pragma unroll
-    for (int i = 0; i < S::kStage; ++i) {
-      const int c = tid + 256 * i, r = c / S::kChunks, chunk = c % S::kChunks;
-      *reinterpret_cast<floatx4*>(lds_k[buffer] + r * S::kKStride + chunk * 16) = stage_k[i];
-      *reinterpret_cast<floatx4*>(lds_v[buffer] + r * S::kVStride + chunk * 16) = stage_v[i];
-    }
+      for (int i = 0; i < S::kStage; ++i) {
+        *reinterpret_cast<floatx4*>(put_k + buffer * (KT * S::kKStride) + i * S::kPass * S::kKStride) = stage_k[i];
+        *reinterpret_cast<floatx4*>(put_v + buffer * (KT * S::kVStride) + i * S::kPass * S::kVStride) = stage_v[i];
+      }
   };
 
   floatx16 o[DP / 32];
   Running run;
-  bool safe = false;
-  for (;;) {
+  // SAFE: what V's infinities and NaN do to a row is decided by what the row sees.
+  auto pass = [&](auto safe) {
+    constexpr bool SAFE = decltype(safe)::value;
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) o[t] = floatx16{};
     run = Running();
-    if (begin < end) {
-      fetch(begin);
-      put(0);
-      unsigned long valid = stage_valid;
-      if (begin + KT < end) fetch(begin + KT);
-      __syncthreads();
-      int buffer = 0;
-      for (int at = begin; at < end; at += KT) {
-        const bool work = at < high;
-        floatx16 s[SUB];
-        if (work) {
+    if (begin >= end) return;
+    look_up(begin);
+    fetch(begin);
+    put(0);
+    unsigned long valid = stage_valid;
+    if (begin + KT < end) fetch(begin + KT);
+    __syncthreads();
+    int buffer = 0;
+    for (int at = begin; at < end; at += KT) {
+      const bool work = at < high;
+      const char* const now_k = lds_k[0] + buffer * (KT * S::kKStride);
+      const char* const now_v = lds_v[0] + buffer * (KT * S::kVStride);
+      floatx16 s[SUB];
+      if (work) {
 #pragma unroll
-          for (int u = 0; u < SUB; ++u) s[u] = scores<T, DP>(lds_k[buffer], 32 * u, q, lane);
-        }
-        const unsigned long next_valid = stage_valid;
-        if (at + KT < end) {
-          put(buffer ^ 1);
-          if (at + 2 * KT < end) fetch(at + 2 * KT);
-        }
-        if (work) {
-          const bool masked = at + KT > low || (PAGED && valid != (KT == 64 ? ~0ul : (1ul << KT) - 1));
-          if (masked) {
-            const int seen = min(limit, end) - at;
-#pragma unroll
-            for (int u = 0; u < SUB; ++u)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int key = 32 * u + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-                if (key >= seen || (PAGED && !(valid >> key & 1))) s[u][i] = -INFINITY;
-              }
-          }
-          softmax_step<T, DP, SUB>(s, o, run, a.scale_log2);
-          if (masked && safe) {
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) weighted_sum<T, DP, true>(lds_v[buffer], 32 * u, s[u], o, lane);
-            add_not_finite<T, DP>(lds_v[buffer], min(min(limit, end) - at, KT), valid, o, lane);
-          } else {
-#pragma unroll
-            for (int u = 0; u < SUB; ++u) weighted_sum<T, DP, false>(lds_v[buffer], 32 * u, s[u], o, lane);
-          }
-        }
-        valid = next_valid;
-        buffer ^= 1;
-        __syncthreads();
+        for (int u = 0; u < SUB; ++u) s[u] = scores<T, DP>(now_k, 32 * u, q, lane);
       }
+      const unsigned long next_valid = stage_valid;
+      if (at + KT < end) {
+        put(buffer ^ 1);
+        if (at + 2 * KT < end) fetch(at + 2 * KT);
+      }
+      if (work) {
+        const bool masked = at + KT > low || (PAGED && valid != kAllValid);
+        if (masked) {
+          const int seen = min(limit, end) - at;
+#pragma unroll
+          for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int key = 32 * u + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
+              if (key >= seen || (PAGED && !(valid >> key & 1))) s[u][i] = -INFINITY;
+            }
+        }
+        softmax_step<T, DP, SUB>(s, o, run, a.scale_log2);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) weighted_sum<T, DP, SAFE>(now_v, 32 * u, s[u], o, lane);
+        if (SAFE) add_not_finite<T, DP>(now_v, min(min(limit, end) - at, KT), valid, o, lane);
+      }
+      valid = next_valid;
+      buffer ^= 1;
+      __syncthreads();
     }
-    // A weight of zero does not keep an infinity or NaN in V's row out of the products.  If
-    // some row's sums are not finite, everything is done once more, with what such values
-    // do to a row decided by what the row sees.
-    if (safe) break;
-    float check = 0.f;
+  };
+  pass(std::false_type());
+  // A weight of zero does not keep an infinity or NaN in V's row out of the products.  If
+  // some row's sums are not finite, everything is done once more, the safe way.
+  float check = 0.f;
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
+  for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) check += 0.f * o[t][i];
-    if (!__syncthreads_or(check != 0.f)) break;  // (0 * inf and 0 * NaN are NaN, which is not 0)
-    safe = true;
-  }
+    for (int i = 0; i < 16; ++i) check += 0.f * o[t][i];
+  if (__syncthreads_or(check != 0.f)) pass(std::true_type());  // (0 * inf and 0 * NaN are NaN, which is not 0)
   store_rows<T, DP, PAGED>(a, o, run, q0 + token, head, piece, all <= a.piece, real, lane);
 }
 

@@ -42,6 +42,13 @@ inline int check_cache(const char* who, const mcPagedCache* c, int type) {
   return 0;
 }
 
+// A kernel forms the offsets of the rows of a tile in 32 bits.
+inline int check_key_stride(const char* who, const char* what, long token_stride, int type) {
+  MC_REQUIRE(token_stride >= 0 && token_stride * static_cast<long>(type_size(type)) <= (1l << 25),
+             "%s: %s: token_stride %ld is negative or above 2^25 bytes", who, what, token_stride);
+  return 0;
+}
+
 inline int check_type(const char* who, int type, int head_dim) {
   MC_REQUIRE(type == MC_TYPE_F32 || type == MC_TYPE_F16 || type == MC_TYPE_BF16,
              "%s: unknown element type %d", who, type);
