@@ -42,22 +42,59 @@ struct AttentionArgs {
   float* partial;  // [pieces][total_q * heads][DP]: sums over a piece's keys, not divided
   float* stats;    // [pieces][total_q * heads][2]: largest score, sum of weights
   int tiles;       // row tiles of one key head
+  int tile_rows;
 };
 
-constexpr int kTileRows = 128;
-
-// Sequence s starts at starts[s] * group / rows + s * gap on a scale of tiles (gap 1 leaves
-// room for its ragged end), or of rows (group = rows = 1, gap 0).  The last s that starts
-// at `at` or before.
-__device__ __forceinline__ int sequence_of_tile(const int* __restrict__ starts, int num, int group,
-                                                int rows, int at, int gap) {
+// The last sequence that starts at row `at` of the packed queries or before it.
+__device__ __forceinline__ int sequence_of_row(const int* __restrict__ starts, int num, int at) {
   int lo = 0, hi = num;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (static_cast<long>(starts[mid]) * group / rows + mid * gap <= at) lo = mid;
+    if (starts[mid] <= at) lo = mid;
     else hi = mid;
   }
   return lo;
+}
+
+// A tile of query rows, found by a whole wavefront (the same in every wavefront).
+struct TileId {
+  int seq;
+  int index;    // of the sequence's tiles; there may be none of this index
+  int q0, q1;   // its queries
+  int k0, k1;   // packed: its keys; paged: k1 is its context
+};
+
+// Tile number `slot` of one key head: sequence s's tiles begin at slot starts[s] * group /
+// rows + s (s leaves room for the ragged ends).  All that describes up to 64 sequences is
+// loaded at once, a sequence per lane; a bisection in memory would wait for one load after
+// another.
+template <bool PAGED>
+__device__ __forceinline__ TileId find_tile(const AttentionArgs& a, int slot, int rows_per_tile) {
+  const int lane = threadIdx.x & 63, group = a.group.d;
+  const auto starts_at = [&](int s) { return static_cast<long>(a.q_starts[s]) * group / rows_per_tile + s; };
+  int lo = 0, n = a.num;
+  while (n > 64) {
+    const int step = (n + 63) / 64, s = lo + lane * step;
+    const int before = __popcll(__ballot(s < lo + n && starts_at(min(s, a.num - 1)) <= slot));
+    const int skip = max(before - 1, 0) * step;
+    lo += skip;
+    n = min(step, n - skip);
+  }
+  const int s = min(lo + lane, a.num - 1);
+  TileId t;
+  const int raw = a.q_starts[s];
+  t.q1 = min(a.q_starts[s + 1], a.total_q);
+  t.k0 = PAGED ? 0 : a.k_starts[s];
+  t.k1 = PAGED ? a.context_lens[s] : a.k_starts[s + 1];
+  const long at = static_cast<long>(raw) * group / rows_per_tile + s;
+  const int chosen = max(__popcll(__ballot(lane < n && at <= slot)) - 1, 0);
+  t.seq = lo + chosen;
+  t.index = __builtin_amdgcn_readlane(static_cast<int>(slot - at), chosen);
+  t.q0 = max(__builtin_amdgcn_readlane(raw, chosen), 0);
+  t.q1 = __builtin_amdgcn_readlane(t.q1, chosen);
+  t.k0 = __builtin_amdgcn_readlane(t.k0, chosen);
+  t.k1 = __builtin_amdgcn_readlane(t.k1, chosen);
+  return t;
 }
 
 // The keys of a sequence, and what its rows see of them.
@@ -67,29 +104,30 @@ struct Keys {
   int offset;  // row i (of the sequence's queries) sees min(count, offset + i) keys
 };
 
+// k0, k1: the sequence's entries of k_starts, or k1 its context.
 template <bool PAGED>
-__device__ __forceinline__ Keys keys_of(const AttentionArgs& a, int seq, int queries) {
+__device__ __forceinline__ Keys keys_of(const AttentionArgs& a, int k0, int k1, int queries) {
   Keys k;
   if (PAGED) {
-    const int context = max(a.context_lens[seq], 0);
+    const int context = max(k1, 0);
     k.first = 0;
     k.count = static_cast<int>(min(static_cast<long>(min(context, a.max_context)),
                                    static_cast<long>(a.table_width) * a.cache.block_size));
     k.offset = context - queries + 1;
   } else {
-    k.first = max(a.k_starts[seq], 0);
-    k.count = max(min(a.k_starts[seq + 1], a.total_k) - k.first, 0);
+    k.first = max(k0, 0);
+    k.count = max(min(k1, a.total_k) - k.first, 0);
     k.offset = k.count - queries + 1;
   }
   if (!a.causal) k.offset = k.count;
   return k;
 }
 
-// Keys that some row of a row's tile sees (tiles start at multiples of kTileRows in a
+// Keys that some row of a row's tile sees (tiles start at multiples of `tile` in a
 // sequence's rows, token by token and head by head of the group; the last row sees most).
 template <bool PAGED>
-__device__ __forceinline__ int keys_of_tile(const AttentionArgs& a, const Keys& k, int row, int rows) {
-  const int last = min(row / kTileRows * kTileRows + kTileRows - 1, rows - 1);
+__device__ __forceinline__ int keys_of_tile(const AttentionArgs& a, const Keys& k, int row, int rows, int tile) {
+  const int last = min(row / tile * tile + tile - 1, rows - 1);
   return max(min(k.count, a.causal ? k.offset + static_cast<int>(a.group.quotient(last)) : k.count), 0);
 }
 

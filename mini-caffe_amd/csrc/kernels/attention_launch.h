@@ -18,12 +18,12 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
   const int lane = threadIdx.x & 63;
   if (at >= static_cast<long>(a.total_q) * a.heads) return;
   const int token = static_cast<int>(at / a.heads), head = static_cast<int>(at - static_cast<long>(token) * a.heads);
-  const int seq = sequence_of_tile(a.q_starts, a.num, 1, 1, token, 0);
+  const int seq = sequence_of_row(a.q_starts, a.num, token);
   const int q0 = max(a.q_starts[seq], 0), q1 = min(a.q_starts[seq + 1], a.total_q);
   const int queries = min(q1 - q0, a.max_q);
   if (token < q0 || token - q0 >= queries) return;
-  const int all = keys_of_tile<true>(a, keys_of<true>(a, seq, q1 - q0), (token - q0) * static_cast<int>(a.group.d) +
-                                     head % static_cast<int>(a.group.d), queries * static_cast<int>(a.group.d));
+  const int all = keys_of_tile<true>(a, keys_of<true>(a, 0, a.context_lens[seq], q1 - q0), (token - q0) * static_cast<int>(a.group.d) +
+                                     head % static_cast<int>(a.group.d), queries * static_cast<int>(a.group.d), a.tile_rows);
   if (all <= a.piece) return;  // written by the one workgroup that had all of its keys
   const int pieces = (all + a.piece - 1) / a.piece;
   const long step = static_cast<long>(a.total_q) * a.heads;
@@ -49,19 +49,20 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
         l == 0.f ? -INFINITY : (m - kLift<T> + log2f(l)) * 0.69314718f;
 }
 
-template <typename T, int DP, bool PAGED>
+template <typename T, int DP, bool PAGED, int W>
 int launch_tiles(AttentionArgs a, hipStream_t st) {
-  constexpr int kKeys = TileShape<T, DP>::kKeys;
+  using S = TileShape<T, DP, W>;
   const long group = a.group.d;
-  a.tiles = static_cast<int>(a.total_q * group / kTileRows) + a.num;
+  a.tile_rows = S::kRows;
+  a.tiles = static_cast<int>(a.total_q * group / S::kRows) + a.num;
   a.pieces = 1;
   a.piece = a.max_context;
   if (PAGED) {
     // too few tiles to fill the GPU: cut the keys, in pieces of at least four tiles of keys
     const long items = static_cast<long>(a.tiles) * a.heads_kv;
-    const int most = std::max(1, a.max_context / (4 * kKeys));
-    const int wanted = static_cast<int>(std::min<long>(std::max<long>(1, 2 * kNumCu / items), most));
-    a.piece = std::max(ceil_div(ceil_div(a.max_context, wanted), kKeys), 1) * kKeys;
+    const int most = std::max(1, a.max_context / (4 * S::kKeys));
+    const int wanted = static_cast<int>(std::min<long>(std::max<long>(1, 8 / W * kNumCu / items), most));
+    a.piece = std::max(ceil_div(ceil_div(a.max_context, wanted), S::kKeys), 1) * S::kKeys;
     a.pieces = std::max(1, ceil_div(a.max_context, a.piece));
     if (a.pieces > 1) {
       const long rows = static_cast<long>(a.total_q) * a.heads * a.pieces;
@@ -73,12 +74,13 @@ int launch_tiles(AttentionArgs a, hipStream_t st) {
   }
   const long blocks = static_cast<long>(a.tiles) * a.heads_kv * a.pieces;
   MC_REQUIRE(blocks <= INT_MAX, "attention: %ld workgroups", blocks);
-  if (!PAGED)
-    attention_tile_kernel<T, DP, Source::kPacked><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
-  else if (a.cache.block_size % TileShape<T, DP>::kPass == 0)
-    attention_tile_kernel<T, DP, Source::kRuns><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
-  else
-    attention_tile_kernel<T, DP, Source::kPaged><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+  const unsigned grid = static_cast<unsigned>(blocks);
+  if constexpr (!PAGED) {
+    attention_tile_kernel<T, DP, Source::kPacked, W><<<grid, 64 * W, 0, st>>>(a);
+  } else {
+    if (a.block.d % S::kRun == 0) attention_tile_kernel<T, DP, Source::kRuns, W><<<grid, 64 * W, 0, st>>>(a);
+    else attention_tile_kernel<T, DP, Source::kPaged, W><<<grid, 64 * W, 0, st>>>(a);
+  }
   MC_LAUNCH_CHECK();
   if (PAGED && a.pieces > 1) {
     attention_join_kernel<T, DP><<<ceil_div(static_cast<long>(a.total_q) * a.heads, 4), 256, 0, st>>>(a);
@@ -87,13 +89,27 @@ int launch_tiles(AttentionArgs a, hipStream_t st) {
   return 0;
 }
 
+// Eight wavefronts share a tile of keys where rows abound: half the copies of keys into LDS.
+// In bf16, 32/8 heads of 128, causal: 8192 tokens 566 us with four, 531 with eight; sequences
+// of 1024, not causal, 417 and 408; of 512, 250 and 253; of 128, 121 and 147 (a tile's unused
+// rows, and a workgroup alone on its CU has nothing to do while it begins and ends).
+template <typename T, int DP, bool PAGED>
+int launch_rows(const AttentionArgs& a, hipStream_t st) {
+  if constexpr (DP * sizeof(T) <= 256) {  // (wider rows leave one wavefront to a SIMD)
+    const long rows = static_cast<long>(a.total_q) * a.group.d;
+    if (rows / a.num >= 4096 && rows * a.heads_kv >= 2l * kNumCu * TileShape<T, DP, 8>::kRows)
+      return launch_tiles<T, DP, PAGED, 8>(a, st);
+  }
+  return launch_tiles<T, DP, PAGED, 4>(a, st);
+}
+
 template <typename T, bool PAGED>
 int launch_type(const AttentionArgs& a, hipStream_t st) {
-  if (a.head_dim <= 64) return launch_tiles<T, 64, PAGED>(a, st);
-  if (a.head_dim <= 96) return launch_tiles<T, 96, PAGED>(a, st);
-  if (a.head_dim <= 128) return launch_tiles<T, 128, PAGED>(a, st);
-  if (a.head_dim <= 192) return launch_tiles<T, 192, PAGED>(a, st);
-  return launch_tiles<T, 256, PAGED>(a, st);
+  if (a.head_dim <= 64) return launch_rows<T, 64, PAGED>(a, st);
+  if (a.head_dim <= 96) return launch_rows<T, 96, PAGED>(a, st);
+  if (a.head_dim <= 128) return launch_rows<T, 128, PAGED>(a, st);
+  if (a.head_dim <= 192) return launch_rows<T, 192, PAGED>(a, st);
+  return launch_rows<T, 256, PAGED>(a, st);
 }
 
 }  // namespace

@@ -41,8 +41,9 @@ struct Product {  // fp16, bf16
   }
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int W = 4>  // W: wavefronts of the workgroup
 struct TileShape {
+  static constexpr int kRows = 32 * W;
   static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
   static constexpr int kKeys = kRowBytes <= 256 ? 64 : 32;     // keys of a tile
   static constexpr int kChunks = kRowBytes / 16;               // 16-byte chunks of a row
@@ -50,43 +51,68 @@ struct TileShape {
   // 16 rows meet all banks; V's rows so that the 4 (16 bits) or 2 (32 bits, four rows
   // apart) row pieces of a read lie side by side modulo 256 bytes.
   static constexpr int kKStride = (kChunks | 1) * 16;
-  static constexpr int kVStride = sizeof(T) == 2 ? ((kRowBytes / 32) | 1) * 32 : kRowBytes + 32;
+  static constexpr int kVStride = sizeof(T) == 2 ? ((kRowBytes / 64) | 1) * 64 : kRowBytes + 32;
   // Staging: a thread carries one chunk (of a power of two, the last ones idle) of kStage rows.
   static constexpr int kLanes = kChunks <= 8 ? 8 : kChunks <= 16 ? 16 : kChunks <= 32 ? 32 : 64;
-  static constexpr int kPass = 256 / kLanes;                   // rows that the workgroup loads at once
+  static constexpr int kRun = 64 / kLanes;                     // rows that a wavefront loads at once
+  static constexpr int kPass = kRun * W;                       // ... and the workgroup
   static constexpr int kStage = kKeys / kPass;
+  // The results go out through LDS, a wavefront's 32 rows at a time.
+  static constexpr int kOutStride = kRowBytes + 16;
+  static constexpr int kTiles = 2 * kKeys * (kKStride + kVStride);
+  static constexpr int kLds = kTiles > 32 * W * kOutStride ? kTiles : 32 * W * kOutStride;
+  static_assert(kKeys % kPass == 0, "a pass over the workgroup loads more than a tile");
 };
 
 // Where the keys are.
 enum class Source {
   kPacked,  // rows of one tensor
-  kRuns,    // a paged cache whose block size is a multiple of kPass: the rows loaded at once
-            // lie in one block, so addresses are scalars plus a fixed offset per thread
+  kRuns,    // a paged cache whose block size is a multiple of kRun: the rows that a wavefront
+            // loads at once lie in one block, so addresses are scalars plus a fixed offset
   kPaged    // any block size: a lane looks a key up
 };
 
-// Scores of 32 keys (rows `base` on of the K tile) against the wavefront's rows.
+// Tells the scheduler to keep `ahead` LDS reads in flight before the products that use them
+// (`reads` per product): it would issue one or two and wait for them.
+template <int PRODUCTS, int READS, int AHEAD>
+__device__ __forceinline__ void read_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 0);  // LDS reads
+#pragma unroll
+  for (int i = 0; i < PRODUCTS - AHEAD; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);            // a product
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
+// Scores of the tile's keys against the wavefront's rows, in blocks of 32 keys.
 template <typename T, int DP>
-__device__ __forceinline__ floatx16 scores(const char* lds_k, int base, const floatx4* q, int lane) {
+__device__ __forceinline__ void scores(const char* lds_k, const floatx4* q, floatx16* c, int lane) {
   using S = TileShape<T, DP>;
-  const char* at = lds_k + (base + (lane & 31)) * S::kKStride + (lane >> 5) * 16;
-  floatx16 c = {};
+  constexpr int SUB = S::kKeys / 32;
+  const char* at = lds_k + (lane & 31) * S::kKStride + (lane >> 5) * 16;
+#pragma unroll
+  for (int u = 0; u < SUB; ++u) c[u] = floatx16{};
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) {
-      const floatx4 a = *reinterpret_cast<const floatx4*>(at + s * 32);
-      c = Product<T>::mma(__builtin_bit_cast(typename Product<T>::vec8, a),
-                          __builtin_bit_cast(typename Product<T>::vec8, q[s]), c);
-    }
+    for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+        const floatx4 a = *reinterpret_cast<const floatx4*>(at + 32 * u * S::kKStride + s * 32);
+        c[u] = Product<T>::mma(__builtin_bit_cast(typename Product<T>::vec8, a),
+                               __builtin_bit_cast(typename Product<T>::vec8, q[s]), c[u]);
+      }
+    read_ahead<SUB * DP / 16, 1, 4>();
   } else {
 #pragma unroll
-    for (int s = 0; s < DP / 8; ++s) {  // 8 values of d: four products of two (half 0's and half 1's)
-      const floatx4 a = *reinterpret_cast<const floatx4*>(at + s * 32);
+    for (int s = 0; s < DP / 8; ++s)  // 8 values of d: four products of two (half 0's and half 1's)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], q[s][e], c, 0, 0, 0);
-    }
+      for (int u = 0; u < SUB; ++u) {
+        const floatx4 a = *reinterpret_cast<const floatx4*>(at + 32 * u * S::kKStride + s * 32);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[u] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], q[s][e], c[u], 0, 0, 0);
+      }
   }
-  return c;
 }
 
 typedef __attribute__((address_space(3))) shortx4 lds_shortx4;
@@ -100,23 +126,23 @@ __device__ __forceinline__ bool finite16(short x, unsigned short exponent) {
   return (static_cast<unsigned short>(x) & exponent) != exponent;
 }
 
-// O^T += V^T P^T for 32 keys (rows `base` on of the V tile), p: the lane's 16 weights.
+// O^T += V^T P^T for the tile's keys, p: the lane's weights.
 // SAFE: infinities and NaN of V count as 0 here.
 template <typename T, int DP, bool SAFE>
-__device__ __forceinline__ void weighted_sum(const char* lds_v, int base, const floatx16& p, floatx16* o,
-                                             int lane) {
+__device__ __forceinline__ void weighted_sum(const char* lds_v, const floatx16* p, floatx16* o, int lane) {
   using S = TileShape<T, DP>;
+  constexpr int SUB = S::kKeys / 32;
   if constexpr (sizeof(T) == 2) {
     constexpr unsigned short kExponent = __is_same(T, bf16_t) ? 0x7f80 : 0x7c00;
-    typename Product<T>::vec8 w[2];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = static_cast<T>(p[i]);
-    const char* at = lds_v + (base + 4 * (lane >> 5) + ((lane & 15) >> 2)) * S::kVStride +
+    const char* at = lds_v + (4 * (lane >> 5) + ((lane & 15) >> 2)) * S::kVStride +
                      (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
+    for (int s = 0; s < 2 * SUB; ++s) {  // 16 keys at a time
+      typename Product<T>::vec8 w;
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int i = 0; i < 8; ++i) w[i] = static_cast<T>(p[s >> 1][8 * (s & 1) + i]);
+#pragma unroll
+      for (int t = 0; t < DP / 32; ++t) {
         const shortx4 lo = column_of_4(at + 16 * s * S::kVStride + 64 * t);
         const shortx4 hi = column_of_4(at + (16 * s + 8) * S::kVStride + 64 * t);
         shortx8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -124,18 +150,22 @@ __device__ __forceinline__ void weighted_sum(const char* lds_v, int base, const 
 #pragma unroll
           for (int e = 0; e < 8; ++e) a[e] = finite16(a[e], kExponent) ? a[e] : short(0);
         }
-        o[t] = Product<T>::mma(__builtin_bit_cast(typename Product<T>::vec8, a), w[s], o[t]);
+        o[t] = Product<T>::mma(__builtin_bit_cast(typename Product<T>::vec8, a), w, o[t]);
       }
+    }
+    if constexpr (!SAFE) read_ahead<SUB * DP / 16, 2, 2>();
   } else {
-    const char* at = lds_v + (base + 4 * (lane >> 5)) * S::kVStride + (lane & 31) * 4;
+    const char* at = lds_v + 4 * (lane >> 5) * S::kVStride + (lane & 31) * 4;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+    for (int u = 0; u < SUB; ++u)
 #pragma unroll
-      for (int t = 0; t < DP / 32; ++t) {
-        float a = *reinterpret_cast<const float*>(at + (8 * (i >> 2) + (i & 3)) * S::kVStride + 128 * t);
-        if constexpr (SAFE) a = __builtin_isfinite(a) ? a : 0.f;
-        o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[i], o[t], 0, 0, 0);
-      }
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int t = 0; t < DP / 32; ++t) {
+          float a = *reinterpret_cast<const float*>(at + (32 * u + 8 * (i >> 2) + (i & 3)) * S::kVStride + 128 * t);
+          if constexpr (SAFE) a = __builtin_isfinite(a) ? a : 0.f;
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, p[u][i], o[t], 0, 0, 0);
+        }
   }
 }
 
@@ -213,69 +243,86 @@ __device__ __forceinline__ void softmax_step(floatx16* s, floatx16* o, Running& 
     }
 }
 
-// The lane's row: out and lse, or its partial sums where the keys are cut into pieces.
-template <typename T, int DP, bool PAGED>
-__device__ __forceinline__ void store_rows(const AttentionArgs& a, const floatx16* o, Running r, int token,
-                                           int head, int piece, bool whole, bool real, int lane) {
-  r.l += __shfl_xor(r.l, 32, 64);
-  if (!real) return;
-  if (PAGED && !whole) {
-    const long at = (static_cast<long>(piece) * a.total_q + token) * a.heads + head;
-    float* to = a.partial + at * DP + 4 * (lane >> 5);
-#pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<floatx4*>(to + 32 * t + 8 * i) =
-            floatx4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
-    if (lane < 32) {
-      a.stats[2 * at] = r.m;
-      a.stats[2 * at + 1] = r.l;
-    }
-    return;
-  }
-  const float inverse = r.l == 0.f ? 0.f : 1.f / r.l;
-  T* out = static_cast<T*>(a.out.data) + token * a.out.token_stride + head * a.out.head_stride + 4 * (lane >> 5);
+// The wavefront's partial sums, where the keys are cut into pieces.
+template <int DP>
+__device__ __forceinline__ void store_partial(const AttentionArgs& a, const floatx16* o, const Running& r,
+                                              int token, int head, int piece, int lane) {
+  const long at = (static_cast<long>(piece) * a.total_q + token) * a.heads + head;
+  float* to = a.partial + at * DP + 4 * (lane >> 5);
 #pragma unroll
   for (int t = 0; t < DP / 32; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (32 * t + 8 * i < a.head_dim) {  // (head_dim is a multiple of 8)
-        typedef T vec4 __attribute__((ext_vector_type(4)));
-        vec4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = static_cast<T>(o[t][4 * i + e] * inverse);
-        *reinterpret_cast<vec4*>(out + 32 * t + 8 * i) = x;
-      }
-  if (a.lse && lane < 32)
-    a.lse[static_cast<long>(head) * a.total_q + token] =
-        r.l == 0.f ? -INFINITY : (r.m - kLift<T> + log2f(r.l)) * 0.69314718f;
+      *reinterpret_cast<floatx4*>(to + 32 * t + 8 * i) =
+          floatx4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
+  if (lane < 32) {
+    a.stats[2 * at] = r.m;
+    a.stats[2 * at + 1] = r.l;
+  }
 }
 
-template <typename T, int DP, Source SRC>
-__global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_tile_kernel(
-    const AttentionArgs a) {
+// out of the wavefront's rows, through its part of LDS: a lane has pieces of 8 (fp32: 16) bytes
+// of one row; written as they are, they would reach memory as eight partial writes per line
+// (24 packed prompts of up to 1500 tokens, 32/8 heads of 128 in bf16: 262 us against 252).
+// Nothing reads them soon, and past the cache they leave its room to the keys (252 -> 238).
+template <typename T, int DP>
+__device__ __forceinline__ void store_out(const AttentionArgs& a, const floatx16* o, float inverse, char* lds,
+                                          int q0, int hk, int first, int rows, int lane) {
   using S = TileShape<T, DP>;
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  char* const mine = lds + (lane & 31) * S::kOutStride + 4 * (lane >> 5) * static_cast<int>(sizeof(T));
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      vec4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = static_cast<T>(o[t][4 * i + e] * inverse);
+      *reinterpret_cast<vec4*>(mine + (32 * t + 8 * i) * static_cast<int>(sizeof(T))) = x;
+    }
+  __builtin_amdgcn_wave_barrier();  // one wavefront's own rows: LDS keeps the order of its accesses
+  constexpr int kChunk = 16 / static_cast<int>(sizeof(T));
+  const int chunk = lane % S::kLanes, group = a.group.d;
+  if (chunk * kChunk < a.head_dim)
+#pragma unroll
+    for (int i = 0; i < 32 / S::kRun; ++i) {
+      const int r = i * S::kRun + lane / S::kLanes, row = first + r;
+      if (row < rows) {
+        const int token = a.group.quotient(row), head = hk * group + (row - token * group);
+        T* out = static_cast<T*>(a.out.data) + (q0 + token) * a.out.token_stride + head * a.out.head_stride;
+        __builtin_nontemporal_store(*reinterpret_cast<const floatx4*>(lds + r * S::kOutStride + chunk * 16),
+                                    reinterpret_cast<floatx4*>(out + chunk * kChunk));
+      }
+    }
+}
+
+template <typename T, int DP, Source SRC, int W>
+__global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attention_tile_kernel(
+    const AttentionArgs a) {
+  using S = TileShape<T, DP, W>;
   constexpr bool PAGED = SRC != Source::kPacked;
   constexpr int KT = S::kKeys, SUB = KT / 32;
-  __shared__ __attribute__((aligned(16))) char lds_k[2][KT * S::kKStride];
-  __shared__ __attribute__((aligned(16))) char lds_v[2][KT * S::kVStride];
+  __shared__ __attribute__((aligned(16))) char lds[S::kLds];
+  char* const lds_k = lds;                        // two tiles of keys
+  char* const lds_v = lds + 2 * KT * S::kKStride;  // ... and of values
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = a.group.d, D = a.head_dim;
   // key heads vary fastest: with workgroups dealt to the XCDs in turn, eight key heads (or
-  // a divisor or multiple of eight) put each one's keys into one XCD's L2.  Tiles run from
-  // the last, which sees most keys, to the first.
+  // a divisor or multiple of eight) put each one's keys into one XCD's L2.
   const int hk = blockIdx.x % a.heads_kv;
   const int rest = blockIdx.x / a.heads_kv;
-  const int piece = rest / a.tiles, tile = a.tiles - 1 - rest % a.tiles;
-  const int seq = sequence_of_tile(a.q_starts, a.num, group, kTileRows, tile, 1);
-  const int q0 = max(a.q_starts[seq], 0), q1 = min(a.q_starts[seq + 1], a.total_q);
+  const int piece = PAGED ? rest / a.tiles : 0;
+  // Tiles run from the last, which sees most keys of a causal sequence, to the first.
+  const TileId tile = find_tile<PAGED>(a, a.tiles - 1 - (rest - piece * a.tiles), S::kRows);
+  // (said to be scalars, or the loop bounds below are vectors)
+  const int seq = __builtin_amdgcn_readfirstlane(tile.seq);
+  const int q0 = __builtin_amdgcn_readfirstlane(tile.q0), q1 = __builtin_amdgcn_readfirstlane(tile.q1);
   const int queries = PAGED ? min(q1 - q0, a.max_q) : q1 - q0;
-  const int first = (tile - static_cast<int>(static_cast<long>(a.q_starts[seq]) * group / kTileRows + seq)) * kTileRows;
-  const int rows = queries * group;
+  const int first = __builtin_amdgcn_readfirstlane(tile.index) * S::kRows, rows = queries * group;
   if (first < 0 || first >= rows) return;  // (tiles are counted generously)
-  const Keys keys = keys_of<PAGED>(a, seq, q1 - q0);
+  const Keys keys = keys_of<PAGED>(a, __builtin_amdgcn_readfirstlane(tile.k0),
+                                   __builtin_amdgcn_readfirstlane(tile.k1), q1 - q0);
 
   // the lane's row; those past the last repeat it and are not stored
   const int row = min(first + 32 * wave + (lane & 31), rows - 1);
@@ -285,10 +332,20 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_
   // rows see more from the first to the last of a wavefront
   const int low = __builtin_amdgcn_readfirstlane(limit);
   const int high = __builtin_amdgcn_readlane(limit, 31);
-  const int all = keys_of_tile<PAGED>(a, keys, first, rows);  // over the workgroup's
+  const int all = keys_of_tile<PAGED>(a, keys, first, rows, S::kRows);  // over the workgroup's
   const int begin = PAGED ? min(piece * a.piece, all) : 0;
   const int end = PAGED ? static_cast<int>(min(static_cast<long>(begin) + a.piece, static_cast<long>(all))) : all;
   if (PAGED && piece > 0 && begin >= all) return;
+
+  // Blocks that do not exist are looked for once; where there is one, every tile asks for its keys.
+  const int* const table = PAGED ? a.block_table + static_cast<long>(seq) * a.table_width : nullptr;
+  bool missing = false;
+  if (PAGED && begin < end) {
+    const int last = a.block.quotient(end - 1);
+    for (int b = a.block.quotient(begin) + tid; b <= last; b += 64 * W)
+      missing |= static_cast<unsigned>(table[b]) >= static_cast<unsigned>(a.cache.num_blocks);
+    missing = __syncthreads_or(missing);
+  }
 
   // queries: 16 bytes per 16 (fp32: 8) values of d, the lane's half of them
   floatx4 q[S::kChunks / 2];
@@ -315,11 +372,11 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_
       static_cast<const T*>(PAGED ? a.cache.values : a.v.data) +
       hk * (PAGED ? a.cache.head_stride : a.v.head_stride) + (PAGED ? 0 : keys.first * a.v.token_stride));
   const unsigned chunk_at = there ? chunk * 16 : 0;
-  const unsigned k_off = pass_row * static_cast<unsigned>(k_stride) + chunk_at;
-  const unsigned v_off = pass_row * static_cast<unsigned>(v_stride) + chunk_at;
-  const int* table = PAGED ? a.block_table + static_cast<long>(seq) * a.table_width : nullptr;
-  char* const put_k = lds_k[0] + pass_row * S::kKStride + chunk * 16;
-  char* const put_v = lds_v[0] + pass_row * S::kVStride + chunk * 16;
+  const int run_row = lane / S::kLanes;  // of the rows that the wavefront loads
+  const unsigned k_off = (SRC == Source::kRuns ? run_row : pass_row) * static_cast<unsigned>(k_stride) + chunk_at;
+  const unsigned v_off = (SRC == Source::kRuns ? run_row : pass_row) * static_cast<unsigned>(v_stride) + chunk_at;
+  char* const put_k = lds_k + pass_row * S::kKStride + chunk * 16;
+  char* const put_v = lds_v + pass_row * S::kVStride + chunk * 16;
   if (S::kLanes != S::kChunks || DP != D) {
     if (!there && chunk < S::kChunks)
 #pragma unroll
@@ -331,13 +388,15 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_
   }
   floatx4 stage_k[S::kStage], stage_v[S::kStage];
   constexpr unsigned long kAllValid = KT == 64 ? ~0ul : (1ul << KT) - 1;
-  unsigned long stage_valid = kAllValid;
   int number[S::kStage];  // kRuns: the next tile's blocks
   auto look_up = [&](int tile_begin) {
     if constexpr (SRC == Source::kRuns)
 #pragma unroll
       for (int i = 0; i < S::kStage; ++i)
-        number[i] = table[a.block.quotient(min(tile_begin + i * S::kPass, end - 1))];
+        number[i] = table[a.block.quotient(min(tile_begin + i * S::kPass + wave * S::kRun, end - 1))];
+  };
+  auto exist = [&](int tile_begin) {  // bit k: the tile's key k has a block
+    return __ballot(cache_row(a, table, min(tile_begin + lane % KT, end - 1)) >= 0) & kAllValid;
   };
   auto fetch = [&](int tile_begin) {  // keys past the end repeat the last one
     if constexpr (SRC == Source::kPacked) {
@@ -359,30 +418,22 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_
         }
       }
     } else if constexpr (SRC == Source::kRuns) {
-      stage_valid = kAllValid;
 #pragma unroll
       for (int i = 0; i < S::kStage; ++i) {
         // (rows past the end lie in the last key's block)
-        const unsigned key = min(tile_begin + i * S::kPass, (end - 1) / S::kPass * S::kPass);
-        int n = number[i];
-        if (static_cast<unsigned>(n) >= static_cast<unsigned>(a.cache.num_blocks)) {
-          n = 0;
-          stage_valid &= ~(((1ul << S::kPass) - 1) << (i * S::kPass));
-        }
+        const unsigned key = min(tile_begin + i * S::kPass + wave * S::kRun, (end - 1) / S::kRun * S::kRun);
+        const int n = static_cast<unsigned>(number[i]) < static_cast<unsigned>(a.cache.num_blocks) ? number[i] : 0;
         const long at = (n * a.cache.block_stride) * static_cast<long>(sizeof(T)) +
                         (key - a.block.quotient(key) * a.block.d) * k_stride;
         unsigned off = k_off;
         if (tile_begin + KT > end)
-          off = min(pass_row, end - 1 - static_cast<int>(key)) * static_cast<unsigned>(k_stride) + chunk_at;
+          off = min(run_row, end - 1 - static_cast<int>(key)) * static_cast<unsigned>(k_stride) + chunk_at;
         stage_k[i] = *reinterpret_cast<const floatx4*>(kbase + at + off);
         stage_v[i] = *reinterpret_cast<const floatx4*>(vbase + at + off);
       }
       if (tile_begin + KT < end) look_up(tile_begin + KT);
     } else {
-      const int key = tile_begin + (lane % KT);
-      long at = cache_row(a, table, min(key, end - 1));
-      stage_valid = __ballot(at >= 0 && key < end) & kAllValid;
-      at = max(at, 0l) * static_cast<long>(sizeof(T)) ;
+      const long at = max(cache_row(a, table, min(tile_begin + lane % KT, end - 1)), 0l) * static_cast<long>(sizeof(T));
 #pragma unroll
       for (int i = 0; i < S::kStage; ++i) {
         const long from = __shfl(at, pass_row + i * S::kPass, 64) + chunk_at;
@@ -412,27 +463,24 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_
     look_up(begin);
     fetch(begin);
     put(0);
-    unsigned long valid = stage_valid;
     if (begin + KT < end) fetch(begin + KT);
     __syncthreads();
     int buffer = 0;
     for (int at = begin; at < end; at += KT) {
       const bool work = at < high;
-      const char* const now_k = lds_k[0] + buffer * (KT * S::kKStride);
-      const char* const now_v = lds_v[0] + buffer * (KT * S::kVStride);
+      const char* const now_k = lds_k + buffer * (KT * S::kKStride);
+      const char* const now_v = lds_v + buffer * (KT * S::kVStride);
       floatx16 s[SUB];
-      if (work) {
-#pragma unroll
-        for (int u = 0; u < SUB; ++u) s[u] = scores<T, DP>(now_k, 32 * u, q, lane);
-      }
-      const unsigned long next_valid = stage_valid;
+      if (work) scores<T, DP>(now_k, q, s, lane);
       if (at + KT < end) {
         put(buffer ^ 1);
         if (at + 2 * KT < end) fetch(at + 2 * KT);
       }
       if (work) {
-        const bool masked = at + KT > low || (PAGED && valid != kAllValid);
+        const bool masked = at + KT > low || (PAGED && missing);
+        unsigned long valid = kAllValid;
         if (masked) {
+          if (PAGED && missing) valid = exist(at);
           const int seen = min(limit, end) - at;
 #pragma unroll
           for (int u = 0; u < SUB; ++u)
@@ -443,11 +491,9 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_
             }
         }
         softmax_step<T, DP, SUB>(s, o, run, a.scale_log2);
-#pragma unroll
-        for (int u = 0; u < SUB; ++u) weighted_sum<T, DP, SAFE>(now_v, 32 * u, s[u], o, lane);
+        weighted_sum<T, DP, SAFE>(now_v, s, o, lane);
         if (SAFE) add_not_finite<T, DP>(now_v, min(min(limit, end) - at, KT), valid, o, lane);
       }
-      valid = next_valid;
       buffer ^= 1;
       __syncthreads();
     }
@@ -461,7 +507,16 @@ __global__ __launch_bounds__(256, DP * sizeof(T) <= 256 ? 2 : 1) void attention_
 #pragma unroll
     for (int i = 0; i < 16; ++i) check += 0.f * o[t][i];
   if (__syncthreads_or(check != 0.f)) pass(std::true_type());  // (0 * inf and 0 * NaN are NaN, which is not 0)
-  store_rows<T, DP, PAGED>(a, o, run, q0 + token, head, piece, all <= a.piece, real, lane);
+  run.l += __shfl_xor(run.l, 32, 64);
+  if (PAGED && all > a.piece) {
+    if (real) store_partial<DP>(a, o, run, q0 + token, head, piece, lane);
+    return;
+  }
+  store_out<T, DP>(a, o, run.l == 0.f ? 0.f : 1.f / run.l, lds + wave * (32 * S::kOutStride), q0, hk,
+                   first + 32 * wave, rows, lane);
+  if (a.lse && real && lane < 32)
+    a.lse[static_cast<long>(head) * a.total_q + q0 + token] =
+        run.l == 0.f ? -INFINITY : (run.m - kLift<T> + log2f(run.l)) * 0.69314718f;
 }
 
 }  // namespace mchip
