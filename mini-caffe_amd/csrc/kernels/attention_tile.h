@@ -388,12 +388,17 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
   }
   floatx4 stage_k[S::kStage], stage_v[S::kStage];
   constexpr unsigned long kAllValid = KT == 64 ? ~0ul : (1ul << KT) - 1;
-  int number[S::kStage];  // kRuns: the next tile's blocks
-  auto look_up = [&](int tile_begin) {
-    if constexpr (SRC == Source::kRuns)
-#pragma unroll
-      for (int i = 0; i < S::kStage; ++i)
-        number[i] = table[a.block.quotient(min(tile_begin + i * S::kPass + wave * S::kRun, end - 1))];
+  // kRuns: 64 entries of the block table, one per lane, from block `window` on, and those 32
+  // further on, asked for long before they are used.  A tile spans 32 blocks at most.
+  static_assert(KT / S::kRun <= 32, "a tile spans more than half a window");
+  const int last_block = SRC == Source::kRuns && begin < end ? a.block.quotient(end - 1) : 0;
+  int window = 0, entry = 0, next_entry = 0;
+  auto open_window = [&](int tile_begin) {
+    if constexpr (SRC == Source::kRuns) {
+      window = a.block.quotient(tile_begin);
+      entry = table[min(window + lane, last_block)];
+      next_entry = table[min(window + 32 + lane, last_block)];
+    }
   };
   auto exist = [&](int tile_begin) {  // bit k: the tile's key k has a block
     return __ballot(cache_row(a, table, min(tile_begin + lane % KT, end - 1)) >= 0) & kAllValid;
@@ -418,20 +423,25 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
         }
       }
     } else if constexpr (SRC == Source::kRuns) {
+      if (static_cast<int>(a.block.quotient(min(tile_begin + KT, end) - 1)) >= window + 64) {
+        window += 32;
+        entry = next_entry;
+        next_entry = table[min(window + 32 + lane, last_block)];
+      }
 #pragma unroll
       for (int i = 0; i < S::kStage; ++i) {
         // (rows past the end lie in the last key's block)
         const unsigned key = min(tile_begin + i * S::kPass + wave * S::kRun, (end - 1) / S::kRun * S::kRun);
-        const int n = static_cast<unsigned>(number[i]) < static_cast<unsigned>(a.cache.num_blocks) ? number[i] : 0;
-        const long at = (n * a.cache.block_stride) * static_cast<long>(sizeof(T)) +
-                        (key - a.block.quotient(key) * a.block.d) * k_stride;
+        const int b = a.block.quotient(key);
+        int n = __builtin_amdgcn_readlane(entry, b - window);
+        n = static_cast<unsigned>(n) < static_cast<unsigned>(a.cache.num_blocks) ? n : 0;
+        const long at = (n * a.cache.block_stride) * static_cast<long>(sizeof(T)) + (key - b * a.block.d) * k_stride;
         unsigned off = k_off;
         if (tile_begin + KT > end)
           off = min(run_row, end - 1 - static_cast<int>(key)) * static_cast<unsigned>(k_stride) + chunk_at;
         stage_k[i] = *reinterpret_cast<const floatx4*>(kbase + at + off);
         stage_v[i] = *reinterpret_cast<const floatx4*>(vbase + at + off);
       }
-      if (tile_begin + KT < end) look_up(tile_begin + KT);
     } else {
       const long at = max(cache_row(a, table, min(tile_begin + lane % KT, end - 1)), 0l) * static_cast<long>(sizeof(T));
 #pragma unroll
@@ -460,7 +470,7 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
     for (int t = 0; t < DP / 32; ++t) o[t] = floatx16{};
     run = Running();
     if (begin >= end) return;
-    look_up(begin);
+    open_window(begin);
     fetch(begin);
     put(0);
     if (begin + KT < end) fetch(begin + KT);
