@@ -43,6 +43,7 @@ struct AttentionArgs {
   float* stats;    // [pieces][total_q * heads][2]: largest score, sum of weights
   int tiles;       // row tiles of one key head
   int tile_rows;
+  int* counters;   // attention_rows.h: [num * heads_kv], zero
 };
 
 // The last sequence that starts at row `at` of the packed queries or before it.

@@ -3,9 +3,10 @@
 #ifndef MCHIP_ATTENTION_LAUNCH_H_
 #define MCHIP_ATTENTION_LAUNCH_H_
 
-#include "attention_tile.h"
+#include "attention_rows.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace mchip {
 namespace {
@@ -58,10 +59,19 @@ int launch_tiles(AttentionArgs a, hipStream_t st) {
   a.pieces = 1;
   a.piece = a.max_context;
   if (PAGED) {
-    // too few tiles to fill the GPU: cut the keys, in pieces of at least four tiles of keys
-    const long items = static_cast<long>(a.tiles) * a.heads_kv;
-    const int most = std::max(1, a.max_context / (4 * S::kKeys));
-    const int wanted = static_cast<int>(std::min<long>(std::max<long>(1, 8 / W * kNumCu / items), most));
+    // Too few tiles to fill the GPU: cut the keys, into the number of pieces whose rounds of
+    // workgroups, each a piece and about five tiles' time to begin and end, take least.  (A
+    // chunk of 512 over 32768, 32/8 heads of 128 in bf16, eight wavefronts: two pieces 537 us,
+    // three 369, four, which give every CU one workgroup, 309, six 395, eight 324.)
+    const long tiles = std::max<long>(ceil_div(a.total_q * group, S::kRows), std::min(a.num, a.total_q));
+    const long items = tiles * a.heads_kv, slots = 8 / W * kNumCu;
+    const int most = std::max(1, std::min(a.max_context / (4 * S::kKeys), 64));
+    int wanted = 1;
+    long best = LONG_MAX;
+    for (int p = 1; p <= most && (p == 1 || items * (p - 1) < 2 * slots); ++p) {
+      const long time = (items * p + slots - 1) / slots * (ceil_div(a.max_context, p) + 5 * S::kKeys);
+      if (time < best) best = time, wanted = p;
+    }
     a.piece = std::max(ceil_div(ceil_div(a.max_context, wanted), S::kKeys), 1) * S::kKeys;
     a.pieces = std::max(1, ceil_div(a.max_context, a.piece));
     if (a.pieces > 1) {
@@ -89,12 +99,41 @@ int launch_tiles(AttentionArgs a, hipStream_t st) {
   return 0;
 }
 
+// At most 32 rows of a key head per request: attention_rows.h.
+template <typename T, int DP, int RB>
+int launch_few_rows(AttentionArgs a, hipStream_t st) {
+  using S = RowsShape<T, DP>;
+  // Pieces: enough for a few rounds of workgroups, so that long and short contexts even out,
+  // of two tiles per wavefront at least.
+  const long items = static_cast<long>(a.num) * a.heads_kv;
+  const int most = std::max(1, ceil_div(a.max_context, 2 * S::kSpan));
+  const int wanted = static_cast<int>(std::min<long>(std::max<long>(1, 8 * kNumCu / items), most));
+  a.piece = std::max(ceil_div(ceil_div(a.max_context, wanted), S::kSpan), 1) * S::kSpan;
+  a.pieces = std::max(1, ceil_div(a.max_context, a.piece));
+  if (a.pieces > 1) {
+    const size_t bytes = static_cast<size_t>(items) * a.pieces * (16 * RB * (DP + 2)) * sizeof(float);
+    if (stream_workspace(st, bytes, &a.partial) || stream_counters(st, static_cast<size_t>(items), &a.counters))
+      return -1;
+  }
+  const long blocks = items * a.pieces;
+  MC_REQUIRE(blocks <= INT_MAX, "attention: %ld workgroups", blocks);
+  attention_rows_kernel<T, DP, RB><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+  MC_LAUNCH_CHECK();
+  return 0;
+}
+
 // Eight wavefronts share a tile of keys where rows abound: half the copies of keys into LDS.
 // In bf16, 32/8 heads of 128, causal: 8192 tokens 566 us with four, 531 with eight; sequences
 // of 1024, not causal, 417 and 408; of 512, 250 and 253; of 128, 121 and 147 (a tile's unused
 // rows, and a workgroup alone on its CU has nothing to do while it begins and ends).
 template <typename T, int DP, bool PAGED>
 int launch_rows(const AttentionArgs& a, hipStream_t st) {
+  if constexpr (PAGED) {
+    const long most = static_cast<long>(std::min(a.max_q, a.total_q)) * a.group.d;
+    if (most <= 16) return launch_few_rows<T, DP, 1>(a, st);
+    if constexpr (DP * sizeof(T) <= 256)  // (wider rows of 32 do not fit the registers)
+      if (most <= 32) return launch_few_rows<T, DP, 2>(a, st);
+  }
   if constexpr (DP * sizeof(T) <= 256) {  // (wider rows leave one wavefront to a SIMD)
     const long rows = static_cast<long>(a.total_q) * a.group.d;
     if (rows / a.num >= 4096 && rows * a.heads_kv >= 2l * kNumCu * TileShape<T, DP, 8>::kRows)

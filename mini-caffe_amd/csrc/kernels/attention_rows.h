@@ -1,0 +1,379 @@
+// Attention of few query rows over a paged cache: single new tokens, and short chunks.
+//
+// A request's rows of one key head (new tokens times the group's heads: at most 16 RB) fit
+// one or two blocks of 16, so the work is to stream keys and values, each read once, and
+// the bound is HBM.  What counts is how much is in flight: the wavefronts of a workgroup
+// take tiles of the keys in turn, each with LDS of its own and no barrier in the loop, and
+// ask for the next tile as soon as one has arrived.  Long contexts are cut into pieces, one
+// workgroup each; the last of a request's workgroups to finish joins them.
+//
+// The products are those of attention_tile.h in 16 x 16 blocks: lane l has row l % 16 and of
+// each 16 keys 4 (l / 16) .. + 4.  In 16 bits one product takes 32 keys, which the lanes hold
+// as two such runs.
+#ifndef MCHIP_ATTENTION_ROWS_H_
+#define MCHIP_ATTENTION_ROWS_H_
+
+#include "attention_tile.h"
+
+namespace mchip {
+
+template <typename T, int DP>
+struct RowsShape {
+  static constexpr int kWaves = 4;
+  static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
+  static constexpr int kKeys = sizeof(T) == 2 || kRowBytes <= 256 ? 32 : 16;  // of a tile
+  static constexpr int kChunks = kRowBytes / 16;
+  // Rows apart so that the lanes of one cycle meet all 64 banks: an odd number of chunks for
+  // K (16 rows, one chunk), of 32 bytes for V in 16 bits (8 rows, 32 bytes each), 16 bytes
+  // more than a multiple of 64 in 32 bits (4 rows, four apart, 64 bytes each).
+  static constexpr int kKStride = (kChunks | 1) * 16;
+  static constexpr int kVStride = sizeof(T) == 2 ? ((kRowBytes / 32) | 1) * 32 : kRowBytes + 16;
+  static constexpr int kLanes = kChunks <= 8 ? 8 : kChunks <= 16 ? 16 : kChunks <= 32 ? 32 : 64;
+  static constexpr int kRun = 64 / kLanes;          // rows of one load
+  static constexpr int kStage = kKeys / kRun;       // loads of K, and of V, per tile
+  static constexpr int kTile = kKeys * (kKStride + kVStride);
+  static constexpr int kSpan = kWaves * kKeys;      // keys that the workgroup takes at once
+};
+
+template <typename T>
+__device__ __forceinline__ floatx4 mma16(floatx4 a, floatx4 b, floatx4 c) {
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  if constexpr (__is_same(T, bf16_t))
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ void store_through(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float load_through(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+template <typename T, int DP, int RB>
+__global__ __launch_bounds__(256, 1) void attention_rows_kernel(const AttentionArgs a) {
+  using S = RowsShape<T, DP>;
+  constexpr int KT = S::kKeys, SUB = KT / 16, W = S::kWaves, DT = DP / 16;
+  constexpr int kOut = 16 * RB * DP * 4;  // a wavefront's sums, on their way to the others
+  constexpr int kMine = S::kTile > kOut ? S::kTile : kOut;
+  __shared__ __attribute__((aligned(16))) char lds[W * kMine];
+  __shared__ float stats[W][16 * RB][2];
+  __shared__ int arrived;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = a.group.d, D = a.head_dim, l16 = lane & 15, l4 = lane >> 4;
+  const int hk = blockIdx.x % a.heads_kv;
+  const int rest = blockIdx.x / a.heads_kv;
+  const int piece = rest / a.num, seq = rest - piece * a.num;
+  const int q0 = max(a.q_starts[seq], 0), q1 = min(a.q_starts[seq + 1], a.total_q);
+  const Keys keys = keys_of<true>(a, 0, a.context_lens[seq], q1 - q0);
+  const int queries = min(q1 - q0, a.max_q), rows = queries * group;
+  if (rows <= 0) return;
+  const int all = keys_of_tile<true>(a, keys, rows - 1, rows, 16 * RB);
+  const int begin = min(piece * a.piece, all);
+  const int end = static_cast<int>(min(static_cast<long>(begin) + a.piece, static_cast<long>(all)));
+  if (piece > 0 && begin >= all) return;
+
+  // the lane's rows; those past the last repeat it and are not stored
+  int limit[RB];
+  floatx4 q[RB][S::kChunks / 4];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int row = min(16 * b + l16, rows - 1);
+    const int token = a.group.quotient(row), head = hk * group + (row - token * group);
+    limit[b] = max(min(keys.count, a.causal ? keys.offset + token : keys.count), 0);
+    const char* at = reinterpret_cast<const char*>(static_cast<const T*>(a.q.data) +
+                                                   (q0 + token) * a.q.token_stride + head * a.q.head_stride);
+#pragma unroll
+    for (int s = 0; s < S::kChunks / 4; ++s) {
+      const int chunk = 4 * s + l4;
+      q[b][s] = floatx4{};
+      if (chunk * static_cast<int>(16 / sizeof(T)) < D) q[b][s] = *reinterpret_cast<const floatx4*>(at + chunk * 16);
+    }
+  }
+  const int low = max(min(keys.count, a.causal ? keys.offset : keys.count), 0);  // the first row's limit
+
+  const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.cache.keys) + hk * a.cache.head_stride);
+  const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.cache.values) + hk * a.cache.head_stride);
+  const int* const table = a.block_table + static_cast<long>(seq) * a.table_width;
+  const int chunk = lane % S::kLanes, run_row = lane / S::kLanes;
+  const bool there = chunk * static_cast<int>(16 / sizeof(T)) < D;
+  const unsigned chunk_at = there ? chunk * 16 : 0;
+  char* const lds_k = lds + wave * kMine;
+  char* const lds_v = lds_k + KT * S::kKStride;
+  char* const put_k = lds_k + run_row * S::kKStride + chunk * 16;
+  char* const put_v = lds_v + run_row * S::kVStride + chunk * 16;
+
+  floatx4 o[RB][DT];
+  Running run[RB];
+  auto pass = [&](auto safe) {
+    constexpr bool SAFE = decltype(safe)::value;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      run[b] = Running();
+#pragma unroll
+      for (int t = 0; t < DT; ++t) o[b][t] = floatx4{};
+    }
+    int at = begin + wave * KT;
+    if (at >= end) return;
+    if (!there && chunk < S::kChunks)  // chunks past head_dim are zero, and not written again
+#pragma unroll
+      for (int i = 0; i < S::kStage; ++i) {
+        *reinterpret_cast<floatx4*>(put_k + i * S::kRun * S::kKStride) = floatx4{};
+        *reinterpret_cast<floatx4*>(put_v + i * S::kRun * S::kVStride) = floatx4{};
+      }
+    floatx4 stage_k[S::kStage], stage_v[S::kStage];
+    // The lane's key of a tile: its block's number is asked for two tiles ahead.
+    auto number_of = [&](int tile) { return table[a.block.quotient(min(tile + lane % KT, end - 1))]; };
+    unsigned long valid, next_valid;
+    auto fetch = [&](int tile, int number) {  // keys past the end repeat the last one
+      const int key = min(tile + lane % KT, end - 1);
+      const bool exists = static_cast<unsigned>(number) < static_cast<unsigned>(a.cache.num_blocks);
+      next_valid = __ballot(exists);
+      const long row = ((exists ? number : 0) * a.cache.block_stride +
+                        static_cast<long>(static_cast<unsigned>(key) - a.block.quotient(key) * a.block.d) *
+                            a.cache.token_stride) * static_cast<long>(sizeof(T));
+#pragma unroll
+      for (int i = 0; i < S::kStage; ++i) {
+        const long from = __shfl(row, i * S::kRun + run_row, 64) + chunk_at;
+        stage_k[i] = *reinterpret_cast<const floatx4*>(kbase + from);
+        stage_v[i] = *reinterpret_cast<const floatx4*>(vbase + from);
+      }
+    };
+    fetch(at, number_of(at));
+    int number = number_of(at + S::kSpan);
+    for (; at < end; at += S::kSpan) {
+      valid = next_valid;
+      if (there)
+#pragma unroll
+        for (int i = 0; i < S::kStage; ++i) {
+          *reinterpret_cast<floatx4*>(put_k + i * S::kRun * S::kKStride) = stage_k[i];
+          *reinterpret_cast<floatx4*>(put_v + i * S::kRun * S::kVStride) = stage_v[i];
+        }
+      if (at + S::kSpan < end) {
+        fetch(at + S::kSpan, number);
+        number = number_of(at + 2 * S::kSpan);
+      }
+      __builtin_amdgcn_wave_barrier();
+      // scores
+      floatx4 s[RB][SUB];
+      const char* const from_k = lds_k + l16 * S::kKStride + l4 * 16;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+        for (int b = 0; b < RB; ++b) s[b][u] = floatx4{};
+#pragma unroll
+        for (int c = 0; c < S::kChunks / 4; ++c) {
+          const floatx4 k = *reinterpret_cast<const floatx4*>(from_k + 16 * u * S::kKStride + c * 64);
+#pragma unroll
+          for (int b = 0; b < RB; ++b) {
+            if constexpr (sizeof(T) == 2) {
+              s[b][u] = mma16<T>(k, q[b][c], s[b][u]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                s[b][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q[b][c][e], s[b][u], 0, 0, 0);
+            }
+          }
+        }
+      }
+      // weights
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        const int seen = min(limit[b], end) - at;
+        if (at + KT > min(low, end) || (valid & ((1ul << KT) - 1)) != (1ul << KT) - 1)
+#pragma unroll
+          for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int key = 16 * u + 4 * l4 + i;
+              if (key >= seen || !(valid >> key & 1)) s[b][u][i] = -INFINITY;
+            }
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = fmaxf(top, s[b][u][i]);
+        top = larger_of_halves(top);
+        top = fmaxf(top, __shfl_xor(top, 16, 64)) * a.scale_log2;
+        Running& r = run[b];
+        if (__any(top > r.m + kSlack<T>)) {
+          const float m = fmaxf(r.m, top);
+          const float keep = m == -INFINITY ? 1.f : exp2f(r.m - m);
+          r.m = m;
+          r.l *= keep;
+#pragma unroll
+          for (int t = 0; t < DT; ++t) o[b][t] *= keep;
+        }
+        const float shift = (r.m == -INFINITY ? 0.f : r.m) - kLift<T>;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[b][u][i] = __builtin_amdgcn_exp2f(fmaf(s[b][u][i], a.scale_log2, -shift));
+            r.l += s[b][u][i];
+          }
+      }
+      // sums of values
+      if constexpr (sizeof(T) == 2) {
+        constexpr unsigned short kExponent = __is_same(T, bf16_t) ? 0x7f80 : 0x7c00;
+        floatx4 w[RB];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          typename Product<T>::vec8 x;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = static_cast<T>(s[b][i >> 2][i & 3]);
+          w[b] = __builtin_bit_cast(floatx4, x);
+        }
+        const char* const from_v = lds_v + (4 * l4 + (l16 >> 2)) * S::kVStride + 8 * (l16 & 3);
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          const shortx4 lo = column_of_4(from_v + 32 * t);
+          const shortx4 hi = column_of_4(from_v + 16 * S::kVStride + 32 * t);
+          shortx8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          if constexpr (SAFE) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = finite16(v[e], kExponent) ? v[e] : short(0);
+          }
+#pragma unroll
+          for (int b = 0; b < RB; ++b) o[b][t] = mma16<T>(__builtin_bit_cast(floatx4, v), w[b], o[b][t]);
+        }
+      } else {
+        const char* const from_v = lds_v + 4 * l4 * S::kVStride + l16 * 4;
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+              float v = *reinterpret_cast<const float*>(from_v + (16 * u + i) * S::kVStride + 64 * t);
+              if constexpr (SAFE) v = __builtin_isfinite(v) ? v : 0.f;
+#pragma unroll
+              for (int b = 0; b < RB; ++b)
+                o[b][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[b][u][i], o[b][t], 0, 0, 0);
+            }
+      }
+      if constexpr (SAFE) {  // see add_not_finite
+#pragma unroll
+        for (int b = 0; b < RB; ++b)
+          for (int key = 0; key < min(min(limit[b], end) - at, KT); ++key) {
+            if (!(valid >> key & 1)) continue;
+            const T* row = reinterpret_cast<const T*>(lds_v + key * S::kVStride);
+#pragma unroll
+            for (int t = 0; t < DT; ++t)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float v = static_cast<float>(row[16 * t + 4 * l4 + i]);
+                if (!__builtin_isfinite(v)) o[b][t][i] += v;
+                __builtin_amdgcn_sched_barrier(0);
+              }
+          }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  };
+  pass(std::false_type());
+  float check = 0.f;
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) check += 0.f * o[b][t][i];
+  if (__any(check != 0.f)) pass(std::true_type());
+
+  // The wavefronts' sums meet in LDS.
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    float l = run[b].l;
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (lane < 16) {
+      stats[wave][16 * b + lane][0] = run[b].m;
+      stats[wave][16 * b + lane][1] = l;
+    }
+    float* const mine = reinterpret_cast<float*>(lds + wave * kMine) + (16 * b + l16) * DP + 4 * l4;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) *reinterpret_cast<floatx4*>(mine + 16 * t) = o[b][t];
+  }
+  __syncthreads();
+  const bool whole = all <= a.piece;
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // values of d per thread: 16 bytes of out
+  auto join = [&](int r, int c, int count, auto stat, auto value, float* m, float* l, float* x) {
+    float top = -INFINITY;
+    for (int p = 0; p < count; ++p) top = fmaxf(top, stat(p, 0));
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = 0.f;
+    for (int p = 0; p < count; ++p) {
+      const float w = exp2f(stat(p, 0) - base);
+      sum += w * stat(p, 1);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[e] += w * value(p, e);
+    }
+    *m = top;
+    *l = sum;
+  };
+  auto finish = [&](int r, int c, float m, float l, const float* x) {
+    const int token = a.group.quotient(r), head = hk * group + (r - token * group);
+    const float inverse = l == 0.f ? 0.f : 1.f / l;
+    typedef T vec __attribute__((ext_vector_type(kPer)));
+    vec y;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) y[e] = static_cast<T>(x[e] * inverse);
+    if (c * kPer < D)
+      *reinterpret_cast<vec*>(static_cast<T*>(a.out.data) + (q0 + token) * a.out.token_stride +
+                              head * a.out.head_stride + c * kPer) = y;
+    if (a.lse && c == 0)
+      a.lse[static_cast<long>(head) * a.total_q + q0 + token] =
+          l == 0.f ? -INFINITY : (m - kLift<T> + log2f(l)) * 0.69314718f;
+  };
+  const int items = rows * S::kChunks;
+  // partial sums of a request's key head: [piece][row][DP], the statistics behind them
+  const long unit = static_cast<long>(16 * RB) * (DP + 2);
+  float* const partial = a.partial + (static_cast<long>(seq) * a.heads_kv + hk) * a.pieces * unit;
+  for (int i = tid; i < items; i += 256) {
+    const int r = i / S::kChunks, c = i % S::kChunks;
+    float m, l, x[kPer];
+    join(r, c, W, [&](int p, int k) { return stats[p][r][k]; },
+         [&](int p, int e) { return reinterpret_cast<const float*>(lds + p * kMine)[r * DP + c * kPer + e]; }, &m, &l, x);
+    if (whole) {
+      finish(r, c, m, l, x);
+    } else {
+      float* to = partial + piece * unit;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) store_through(to + r * DP + c * kPer + e, x[e]);
+      if (c == 0) {
+        store_through(to + 16 * RB * DP + 2 * r, m);
+        store_through(to + 16 * RB * DP + 2 * r + 1, l);
+      }
+    }
+  }
+  if (whole) return;
+  // The last workgroup to arrive joins the pieces, in their order.  Partial sums and counter
+  // are accessed at device scope only, past the L2 of an XCD: a workgroup's stores have been
+  // acknowledged by the memory that all XCDs share before it counts.  (gfx950: a device-scope
+  // store is written through and counted by vmcnt until then; the language promises no such
+  // order for relaxed accesses.)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int* const counter = a.counters + static_cast<long>(seq) * a.heads_kv + hk;
+  if (tid == 0) arrived = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  const int pieces = (all + a.piece - 1) / a.piece;
+  if (arrived != pieces - 1) return;
+  if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int i = tid; i < items; i += 256) {
+    const int r = i / S::kChunks, c = i % S::kChunks;
+    float m, l, x[kPer];
+    join(r, c, pieces, [&](int p, int k) { return load_through(partial + p * unit + 16 * RB * DP + 2 * r + k); },
+         [&](int p, int e) { return load_through(partial + p * unit + r * DP + c * kPer + e); }, &m, &l, x);
+    finish(r, c, m, l, x);
+  }
+}
+
+}  // namespace mchip
+
+#endif  // MCHIP_ATTENTION_ROWS_H_
