@@ -103,11 +103,13 @@ int launch_tiles(AttentionArgs a, hipStream_t st) {
 template <typename T, int DP, int RB>
 int launch_few_rows(AttentionArgs a, hipStream_t st) {
   using S = RowsShape<T, DP>;
-  // Pieces: enough for a few rounds of workgroups, so that long and short contexts even out,
-  // of two tiles per wavefront at least.
+  // Pieces: enough for three rounds of workgroups (two or three to a CU, one where rows are
+  // wide), so that long and short contexts even out, of two tiles per wavefront at least.  In
+  // bf16, with 3/4/6/8 times as many workgroups as CUs: 64 x 8192, 32/8 heads of 128 250/237/
+  // 237/238 us; 10 x 20000, 16/2 of 64 23/22/24/31; 9 x 3089, 24/12 of 256 51/59/63/63.
   const long items = static_cast<long>(a.num) * a.heads_kv;
-  const int most = std::max(1, ceil_div(a.max_context, 2 * S::kSpan));
-  const int wanted = static_cast<int>(std::min<long>(std::max<long>(1, 8 * kNumCu / items), most));
+  const int most = std::min(std::max(1, ceil_div(a.max_context, 2 * S::kSpan)), kMaxPieces);
+  const int wanted = static_cast<int>(std::min<long>(std::max<long>(1, (S::kRowBytes <= 256 ? 6 : 3) * kNumCu / items), most));
   a.piece = std::max(ceil_div(ceil_div(a.max_context, wanted), S::kSpan), 1) * S::kSpan;
   a.pieces = std::max(1, ceil_div(a.max_context, a.piece));
   if (a.pieces > 1) {
@@ -122,21 +124,24 @@ int launch_few_rows(AttentionArgs a, hipStream_t st) {
   return 0;
 }
 
-// Eight wavefronts share a tile of keys where rows abound: half the copies of keys into LDS.
-// In bf16, 32/8 heads of 128, causal: 8192 tokens 566 us with four, 531 with eight; sequences
-// of 1024, not causal, 417 and 408; of 512, 250 and 253; of 128, 121 and 147 (a tile's unused
-// rows, and a workgroup alone on its CU has nothing to do while it begins and ends).
+// Eight wavefronts share a tile of keys where rows and keys abound: half the copies of keys
+// into LDS.  In bf16, 32/8 heads of 128: 8192 causal tokens 566 us with four, 531 with eight; a
+// chunk of 512 over 32768 334 and 309; sequences of 1024, not causal, 417 and 408; of 512, 250
+// and 253; of 128, 121 and 147 (a tile's unused rows, and a workgroup alone on its CU has
+// nothing to do while it begins and ends).
 template <typename T, int DP, bool PAGED>
 int launch_rows(const AttentionArgs& a, hipStream_t st) {
+  const long group = a.group.d;
   if constexpr (PAGED) {
-    const long most = static_cast<long>(std::min(a.max_q, a.total_q)) * a.group.d;
+    const long most = std::min(a.max_q, a.total_q) * group;
     if (most <= 16) return launch_few_rows<T, DP, 1>(a, st);
     if constexpr (DP * sizeof(T) <= 256)  // (wider rows of 32 do not fit the registers)
       if (most <= 32) return launch_few_rows<T, DP, 2>(a, st);
   }
   if constexpr (DP * sizeof(T) <= 256) {  // (wider rows leave one wavefront to a SIMD)
-    const long rows = static_cast<long>(a.total_q) * a.group.d;
-    if (rows / a.num >= 4096 && rows * a.heads_kv >= 2l * kNumCu * TileShape<T, DP, 8>::kRows)
+    const long rows = a.total_q * group, keys = PAGED ? a.max_context : a.total_k / a.num;
+    if (rows / a.num >= 1024 && keys >= 1024 &&
+        (PAGED || rows * a.heads_kv >= 2l * kNumCu * TileShape<T, DP, 8>::kRows))
       return launch_tiles<T, DP, PAGED, 8>(a, st);
   }
   return launch_tiles<T, DP, PAGED, 4>(a, st);

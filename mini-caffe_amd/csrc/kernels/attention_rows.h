@@ -44,19 +44,28 @@ __device__ __forceinline__ floatx4 mma16(floatx4 a, floatx4 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec8, a), __builtin_bit_cast(vec8, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ void store_through(float* p, float v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+
+// Two floats at device scope, past the L2 of an XCD.
+__device__ __forceinline__ void store_through(float* p, float x, float y) {
+  __hip_atomic_store(reinterpret_cast<unsigned long*>(p), __builtin_bit_cast(unsigned long, (floatx2{x, y})),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ float load_through(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ floatx2 load_through(const float* p) {
+  return __builtin_bit_cast(floatx2, __hip_atomic_load(reinterpret_cast<const unsigned long*>(p), __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT));
 }
+
+constexpr int kMaxPieces = 128;
 
 template <typename T, int DP, int RB>
 __global__ __launch_bounds__(256, 1) void attention_rows_kernel(const AttentionArgs a) {
   using S = RowsShape<T, DP>;
   constexpr int KT = S::kKeys, SUB = KT / 16, W = S::kWaves, DT = DP / 16;
   constexpr int kOut = 16 * RB * DP * 4;  // a wavefront's sums, on their way to the others
+  constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // values of 16 bytes
   constexpr int kMine = S::kTile > kOut ? S::kTile : kOut;
+  static_assert((kPer + 2) * 256 * 4 <= W * kMine, "the join's sums do not fit");
   __shared__ __attribute__((aligned(16))) char lds[W * kMine];
   __shared__ float stats[W][16 * RB][2];
   __shared__ int arrived;
@@ -66,6 +75,12 @@ __global__ __launch_bounds__(256, 1) void attention_rows_kernel(const AttentionA
   const int hk = blockIdx.x % a.heads_kv;
   const int rest = blockIdx.x / a.heads_kv;
   const int piece = rest / a.num, seq = rest - piece * a.num;
+  const int* const table = a.block_table + static_cast<long>(seq) * a.table_width;
+  // The lane's key of the first tile: its block's number is asked for before it is known
+  // whether the context reaches that far.
+  const unsigned first_block = a.block.quotient(
+      min(static_cast<long>(piece) * a.piece + wave * KT + lane % KT, static_cast<long>(INT_MAX)));
+  const int first_number = table[min(first_block, static_cast<unsigned>(a.table_width - 1))];
   const int q0 = max(a.q_starts[seq], 0), q1 = min(a.q_starts[seq + 1], a.total_q);
   const Keys keys = keys_of<true>(a, 0, a.context_lens[seq], q1 - q0);
   const int queries = min(q1 - q0, a.max_q), rows = queries * group;
@@ -89,16 +104,15 @@ __global__ __launch_bounds__(256, 1) void attention_rows_kernel(const AttentionA
     for (int s = 0; s < S::kChunks / 4; ++s) {
       const int chunk = 4 * s + l4;
       q[b][s] = floatx4{};
-      if (chunk * static_cast<int>(16 / sizeof(T)) < D) q[b][s] = *reinterpret_cast<const floatx4*>(at + chunk * 16);
+      if (chunk * kPer < D) q[b][s] = *reinterpret_cast<const floatx4*>(at + chunk * 16);
     }
   }
   const int low = max(min(keys.count, a.causal ? keys.offset : keys.count), 0);  // the first row's limit
 
   const char* kbase = reinterpret_cast<const char*>(static_cast<const T*>(a.cache.keys) + hk * a.cache.head_stride);
   const char* vbase = reinterpret_cast<const char*>(static_cast<const T*>(a.cache.values) + hk * a.cache.head_stride);
-  const int* const table = a.block_table + static_cast<long>(seq) * a.table_width;
   const int chunk = lane % S::kLanes, run_row = lane / S::kLanes;
-  const bool there = chunk * static_cast<int>(16 / sizeof(T)) < D;
+  const bool there = chunk * kPer < D;
   const unsigned chunk_at = there ? chunk * 16 : 0;
   char* const lds_k = lds + wave * kMine;
   char* const lds_v = lds_k + KT * S::kKStride;
@@ -141,7 +155,7 @@ __global__ __launch_bounds__(256, 1) void attention_rows_kernel(const AttentionA
         stage_v[i] = *reinterpret_cast<const floatx4*>(vbase + from);
       }
     };
-    fetch(at, number_of(at));
+    fetch(at, __shfl(first_number, min(lane % KT, end - 1 - at), 64));
     int number = number_of(at + S::kSpan);
     for (; at < end; at += S::kSpan) {
       valid = next_valid;
@@ -199,8 +213,8 @@ __global__ __launch_bounds__(256, 1) void attention_rows_kernel(const AttentionA
         top = fmaxf(top, __shfl_xor(top, 16, 64)) * a.scale_log2;
         Running& r = run[b];
         if (__any(top > r.m + kSlack<T>)) {
-          const float m = fmaxf(r.m, top);
-          const float keep = m == -INFINITY ? 1.f : exp2f(r.m - m);
+          const float m = top > r.m + kSlack<T> ? top : r.m;  // (see softmax_step)
+          const float keep = m == r.m ? 1.f : exp2f(r.m - m);
           r.m = m;
           r.l *= keep;
 #pragma unroll
@@ -299,23 +313,6 @@ __global__ __launch_bounds__(256, 1) void attention_rows_kernel(const AttentionA
   }
   __syncthreads();
   const bool whole = all <= a.piece;
-  constexpr int kPer = 16 / static_cast<int>(sizeof(T));  // values of d per thread: 16 bytes of out
-  auto join = [&](int r, int c, int count, auto stat, auto value, float* m, float* l, float* x) {
-    float top = -INFINITY;
-    for (int p = 0; p < count; ++p) top = fmaxf(top, stat(p, 0));
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] = 0.f;
-    for (int p = 0; p < count; ++p) {
-      const float w = exp2f(stat(p, 0) - base);
-      sum += w * stat(p, 1);
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) x[e] += w * value(p, e);
-    }
-    *m = top;
-    *l = sum;
-  };
   auto finish = [&](int r, int c, float m, float l, const float* x) {
     const int token = a.group.quotient(r), head = hk * group + (r - token * group);
     const float inverse = l == 0.f ? 0.f : 1.f / l;
@@ -332,23 +329,28 @@ __global__ __launch_bounds__(256, 1) void attention_rows_kernel(const AttentionA
   };
   const int items = rows * S::kChunks;
   // partial sums of a request's key head: [piece][row][DP], the statistics behind them
-  const long unit = static_cast<long>(16 * RB) * (DP + 2);
-  float* const partial = a.partial + (static_cast<long>(seq) * a.heads_kv + hk) * a.pieces * unit;
+  constexpr long kUnit = 16l * RB * (DP + 2);
+  float* const partial = a.partial + (static_cast<long>(seq) * a.heads_kv + hk) * a.pieces * kUnit;
   for (int i = tid; i < items; i += 256) {
     const int r = i / S::kChunks, c = i % S::kChunks;
-    float m, l, x[kPer];
-    join(r, c, W, [&](int p, int k) { return stats[p][r][k]; },
-         [&](int p, int e) { return reinterpret_cast<const float*>(lds + p * kMine)[r * DP + c * kPer + e]; }, &m, &l, x);
+    float m = -INFINITY, l = 0.f, x[kPer] = {};
+#pragma unroll
+    for (int w = 0; w < W; ++w) m = fmaxf(m, stats[w][r][0]);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float weight = exp2f(stats[w][r][0] - (m == -INFINITY ? 0.f : m));
+      l += weight * stats[w][r][1];
+      const float* from = reinterpret_cast<const float*>(lds + w * kMine) + r * DP + c * kPer;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[e] += weight * from[e];
+    }
     if (whole) {
       finish(r, c, m, l, x);
     } else {
-      float* to = partial + piece * unit;
+      float* to = partial + piece * kUnit;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) store_through(to + r * DP + c * kPer + e, x[e]);
-      if (c == 0) {
-        store_through(to + 16 * RB * DP + 2 * r, m);
-        store_through(to + 16 * RB * DP + 2 * r + 1, l);
-      }
+      for (int e = 0; e < kPer; e += 2) store_through(to + r * DP + c * kPer + e, x[e], x[e + 1]);
+      if (c == 0) store_through(to + 16 * RB * DP + 2 * r, m, l);
     }
   }
   if (whole) return;
@@ -365,12 +367,63 @@ __global__ __launch_bounds__(256, 1) void attention_rows_kernel(const AttentionA
   const int pieces = (all + a.piece - 1) / a.piece;
   if (arrived != pieces - 1) return;
   if (tid == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  // 16 bytes of out per thread, and where threads are left the pieces shared among them; all
+  // loads of eight pieces at once (one after another, 76 pieces took 60 us, and the statistics
+  // ahead of the sums 2 us more than together).  Then the shares meet in LDS.
+  const int shares = max(256 / items, 1);
+  float* const sums = reinterpret_cast<float*>(lds);  // [kPer + 2][256]
+  for (int i = tid; i < items * shares; i += 256) {
+    const int item = i % items, share = i / items, r = item / S::kChunks, c = item % S::kChunks;
+    float m = -INFINITY, l = 0.f, x[kPer] = {};
+    constexpr int kAhead = 8;
+    for (int p0 = share; p0 < pieces; p0 += kAhead * shares) {
+      floatx2 y[kAhead][kPer / 2], stat[kAhead];
+#pragma unroll
+      for (int p = 0; p < kAhead; ++p) {
+        const float* from = partial + min(p0 + p * shares, pieces - 1) * kUnit;
+        stat[p] = load_through(from + 16 * RB * DP + 2 * r);
+#pragma unroll
+        for (int e = 0; e < kPer / 2; ++e) y[p][e] = load_through(from + r * DP + c * kPer + 2 * e);
+      }
+      float top = m;
+#pragma unroll
+      for (int p = 0; p < kAhead; ++p) top = fmaxf(top, stat[p][0]);  // (the last piece again: no matter)
+      const float base = top == -INFINITY ? 0.f : top, keep = exp2f(m - base);
+      m = top;
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[e] *= keep;
+#pragma unroll
+      for (int p = 0; p < kAhead; ++p)
+        if (p0 + p * shares < pieces) {
+          const float weight = exp2f(stat[p][0] - base);
+          l += weight * stat[p][1];
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) x[e] += weight * y[p][e >> 1][e & 1];
+        }
+    }
+    if (shares == 1) {
+      finish(r, c, m, l, x);
+    } else {
+      sums[i] = m;
+      sums[256 + i] = l;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) sums[(2 + e) * 256 + i] = x[e];
+    }
+  }
+  if (shares == 1) return;
+  __syncthreads();
   for (int i = tid; i < items; i += 256) {
-    const int r = i / S::kChunks, c = i % S::kChunks;
-    float m, l, x[kPer];
-    join(r, c, pieces, [&](int p, int k) { return load_through(partial + p * unit + 16 * RB * DP + 2 * r + k); },
-         [&](int p, int e) { return load_through(partial + p * unit + r * DP + c * kPer + e); }, &m, &l, x);
-    finish(r, c, m, l, x);
+    float m = -INFINITY, l = 0.f, x[kPer] = {};
+    for (int share = 0; share < shares; ++share) m = fmaxf(m, sums[share * items + i]);
+    for (int share = 0; share < shares; ++share) {
+      const int from = share * items + i;
+      const float weight = exp2f(sums[from] - (m == -INFINITY ? 0.f : m));
+      l += weight * sums[256 + from];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[e] += weight * sums[(2 + e) * 256 + from];
+    }
+    finish(i / S::kChunks, i % S::kChunks, m, l, x);
   }
 }
 

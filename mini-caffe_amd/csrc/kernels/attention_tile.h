@@ -45,7 +45,7 @@ template <typename T, int DP, int W = 4>  // W: wavefronts of the workgroup
 struct TileShape {
   static constexpr int kRows = 32 * W;
   static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
-  static constexpr int kKeys = kRowBytes <= 256 ? 64 : 32;     // keys of a tile
+  static constexpr int kKeys = sizeof(T) == 2 && kRowBytes <= 256 ? 64 : 32;  // keys of a tile
   static constexpr int kChunks = kRowBytes / 16;               // 16-byte chunks of a row
   // LDS rows: an odd number of chunks apart for K, so that 16 lanes that read one chunk of
   // 16 rows meet all banks; V's rows so that the 4 (16 bits) or 2 (32 bits, four rows
@@ -226,8 +226,9 @@ __device__ __forceinline__ void softmax_step(floatx16* s, floatx16* o, Running& 
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
   top = larger_of_halves(top) * scale_log2;
   if (__any(top > r.m + kSlack<T>)) {
-    const float m = fmaxf(r.m, top);
-    const float keep = m == -INFINITY ? 1.f : exp2f(r.m - m);
+    // (only the rows that need it: a row's bits do not depend on what its neighbours hold)
+    const float m = top > r.m + kSlack<T> ? top : r.m;
+    const float keep = m == r.m ? 1.f : exp2f(r.m - m);
     r.m = m;
     r.l *= keep;
 #pragma unroll
@@ -337,16 +338,7 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
   const int end = PAGED ? static_cast<int>(min(static_cast<long>(begin) + a.piece, static_cast<long>(all))) : all;
   if (PAGED && piece > 0 && begin >= all) return;
 
-  // Blocks that do not exist are looked for once; where there is one, every tile asks for its keys.
   const int* const table = PAGED ? a.block_table + static_cast<long>(seq) * a.table_width : nullptr;
-  bool missing = false;
-  if (PAGED && begin < end) {
-    const int last = a.block.quotient(end - 1);
-    for (int b = a.block.quotient(begin) + tid; b <= last; b += 64 * W)
-      missing |= static_cast<unsigned>(table[b]) >= static_cast<unsigned>(a.cache.num_blocks);
-    missing = __syncthreads_or(missing);
-  }
-
   // queries: 16 bytes per 16 (fp32: 8) values of d, the lane's half of them
   floatx4 q[S::kChunks / 2];
   {
@@ -394,7 +386,7 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
   const int last_block = SRC == Source::kRuns && begin < end ? a.block.quotient(end - 1) : 0;
   int window = 0, entry = 0, next_entry = 0;
   auto open_window = [&](int tile_begin) {
-    if constexpr (SRC == Source::kRuns) {
+    if (SRC == Source::kRuns && begin < end) {
       window = a.block.quotient(tile_begin);
       entry = table[min(window + lane, last_block)];
       next_entry = table[min(window + 32 + lane, last_block)];
@@ -461,6 +453,17 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
       }
   };
 
+  open_window(begin);
+  // Blocks that do not exist are looked for once; where there is one, every tile asks for its keys.
+  bool missing = false;
+  if (PAGED && begin < end) {
+    const int last = a.block.quotient(end - 1);
+    for (int b = a.block.quotient(begin) + tid; b <= last; b += 64 * W)
+      missing |= static_cast<unsigned>(table[b]) >= static_cast<unsigned>(a.cache.num_blocks);
+  }
+  if (begin < end) fetch(begin);  // (asked for before the wavefronts wait for each other)
+  if (PAGED && begin < end) missing = __syncthreads_or(missing);
+
   floatx16 o[DP / 32];
   Running run;
   // SAFE: what V's infinities and NaN do to a row is decided by what the row sees.
@@ -470,8 +473,10 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
     for (int t = 0; t < DP / 32; ++t) o[t] = floatx16{};
     run = Running();
     if (begin >= end) return;
-    open_window(begin);
-    fetch(begin);
+    if (SAFE) {
+      open_window(begin);
+      fetch(begin);
+    }
     put(0);
     if (begin + KT < end) fetch(begin + KT);
     __syncthreads();
