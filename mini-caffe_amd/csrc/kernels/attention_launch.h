@@ -138,12 +138,18 @@ int launch_rows(const AttentionArgs& a, hipStream_t st) {
     if constexpr (DP * sizeof(T) <= 256)  // (wider rows of 32 do not fit the registers)
       if (most <= 32) return launch_few_rows<T, DP, 2>(a, st);
   }
-  if constexpr (DP * sizeof(T) <= 256) {  // (wider rows leave one wavefront to a SIMD)
-    const long rows = a.total_q * group, keys = PAGED ? a.max_context : a.total_k / a.num;
+  const long rows = a.total_q * group, keys = PAGED ? a.max_context : a.total_k / a.num;
+  if constexpr (sizeof(T) == 2 && DP <= 128) {  // (wider rows leave one wavefront to a SIMD)
     if (rows / a.num >= 1024 && keys >= 1024 &&
         (PAGED || rows * a.heads_kv >= 2l * kNumCu * TileShape<T, DP, 8>::kRows))
       return launch_tiles<T, DP, PAGED, 8>(a, st);
   }
+  // fp32 by terms of more than 64 values has one tile in LDS with four wavefronts and two with
+  // eight: 4096 causal tokens, 32/8 heads of 128 721 us and 625; five images of 273 to 1369 cells,
+  // 12 heads 191 and 172; three of 100 to 300 39 and 43.  (64 values: 4096 twice, 12 heads, not
+  // causal, 548 and 588.)
+  if constexpr (sizeof(T) == 4 && DP > 64 && DP <= 128)
+    if (rows / a.num >= 512 && keys >= 512) return launch_tiles<T, DP, PAGED, 8>(a, st);
   return launch_tiles<T, DP, PAGED, 4>(a, st);
 }
 

@@ -15,6 +15,11 @@
 // the order of its registers, taken as the ones it supplies to the second, and V's rows
 // are fetched in that order.  16-bit V is transposed on its way out of LDS
 // (ds_read_b64_tr_b16: of 16 lanes that address 4 rows of 16 values, each gets a column).
+//
+// fp32 rows of at most 128 values: each value is the sum of three bf16, x = h + m + l exact to
+// its last bit, and a product the six of them that reach 2^-24 of it (h h', h m', m h', m m',
+// h l', l h'; what is left out, m l' and l m', is below 2^-23 each and 2^-26 on the whole), on the matrix unit's bf16 rate, sixteen times
+// that of fp32.  The terms are formed on the way into LDS, once per workgroup.
 #ifndef MCHIP_ATTENTION_TILE_H_
 #define MCHIP_ATTENTION_TILE_H_
 
@@ -57,9 +62,18 @@ struct TileShape {
   static constexpr int kRun = 64 / kLanes;                     // rows that a wavefront loads at once
   static constexpr int kPass = kRun * W;                       // ... and the workgroup
   static constexpr int kStage = kKeys / kPass;
+  // fp32 by three bf16 terms: a plane of rows for each.
+  static constexpr bool kSplit = sizeof(T) == 4 && DP <= 128;
+  static constexpr int kKPlane = kKeys * ((DP * 2 / 16) | 1) * 16, kVPlane = kKeys * ((DP * 2 / 64) | 1) * 64;
+  static constexpr int kKTile = kSplit ? 3 * kKPlane : kKeys * kKStride;
+  static constexpr int kVTile = kSplit ? 3 * kVPlane : kKeys * kVStride;
+  static_assert(kKTile >= kKeys * kKStride && kVTile >= kKeys * kVStride, "values as they are do not fit their terms' place");
   // The results go out through LDS, a wavefront's 32 rows at a time.
   static constexpr int kOutStride = kRowBytes + 16;
-  static constexpr int kTiles = 2 * kKeys * (kKStride + kVStride);
+  // Two tiles in LDS, one read while the other is written; one where two would leave a CU to a
+  // single workgroup of four wavefronts (terms of 96 and 128 values).
+  static constexpr int kBuffers = kSplit && DP > 64 && W < 8 ? 1 : 2;
+  static constexpr int kTiles = kBuffers * (kKTile + kVTile);
   static constexpr int kLds = kTiles > 32 * W * kOutStride ? kTiles : 32 * W * kOutStride;
   static_assert(kKeys % kPass == 0, "a pass over the workgroup loads more than a tile");
 };
@@ -83,6 +97,60 @@ __device__ __forceinline__ void read_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
   }
   __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
+typedef unsigned uintx2 __attribute__((ext_vector_type(2)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+
+// The three terms of two values, a pair of bf16 each: the upper half of a value as it is (so
+// that no finite value becomes infinite), then twice the rest rounded.  Infinities and NaN
+// give NaN in the second term, and so in every sum they enter.
+struct Terms {
+  unsigned t[3];
+};
+__device__ __forceinline__ Terms terms_of(float x, float y) {
+  Terms r;
+  const unsigned a = __builtin_bit_cast(unsigned, x), b = __builtin_bit_cast(unsigned, y);
+  r.t[0] = __builtin_amdgcn_perm(b, a, 0x07060302);
+  x -= __builtin_bit_cast(float, a & 0xffff0000u);  // exact
+  y -= __builtin_bit_cast(float, b & 0xffff0000u);
+  r.t[1] = __builtin_bit_cast(unsigned, (bf16x2{static_cast<bf16_t>(x), static_cast<bf16_t>(y)}));
+  x -= __builtin_bit_cast(float, r.t[1] << 16);  // exact
+  y -= __builtin_bit_cast(float, r.t[1] & 0xffff0000u);
+  r.t[2] = __builtin_bit_cast(unsigned, (bf16x2{static_cast<bf16_t>(x), static_cast<bf16_t>(y)}));
+  return r;
+}
+
+// c += a b for operands of three terms, the small products first.
+__device__ __forceinline__ floatx16 mma_terms(const uintx4* a, const uintx4* b, floatx16 c) {
+  const auto product = [&](int i, int j) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a[i]), __builtin_bit_cast(bf16x8, b[j]), c, 0, 0, 0);
+  };
+  product(2, 0);
+  product(0, 2);
+  product(1, 1);
+  product(1, 0);
+  product(0, 1);
+  product(0, 0);
+  return c;
+}
+
+// scores() and weighted_sum() by terms.  q: [DP / 16][3].
+template <int DP>
+__device__ __forceinline__ void scores_by_terms(const char* lds_k, const uintx4 (*q)[3], floatx16* c, int lane) {
+  using S = TileShape<float, DP>;
+  constexpr int kStride = S::kKPlane / S::kKeys;
+  const char* at = lds_k + (lane & 31) * kStride + (lane >> 5) * 16;
+  c[0] = floatx16{};
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    uintx4 k[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) k[i] = *reinterpret_cast<const uintx4*>(at + i * S::kKPlane + s * 32);
+    c[0] = mma_terms(k, q[s], c[0]);
+  }
 }
 
 // Scores of the tile's keys against the wavefront's rows, in blocks of 32 keys.
@@ -169,6 +237,35 @@ __device__ __forceinline__ void weighted_sum(const char* lds_v, const floatx16* 
   }
 }
 
+template <int DP>
+__device__ __forceinline__ void weighted_sum_by_terms(const char* lds_v, const floatx16& p, floatx16* o, int lane) {
+  using S = TileShape<float, DP>;
+  constexpr int kStride = S::kVPlane / S::kKeys;
+  const char* at = lds_v + (4 * (lane >> 5) + ((lane & 15) >> 2)) * kStride + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {  // 16 keys at a time
+    uintx4 w[3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const Terms x = terms_of(p[8 * s + 2 * e], p[8 * s + 2 * e + 1]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) w[i][e] = x.t[i];
+    }
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t) {
+      uintx4 v[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const char* from = at + i * S::kVPlane + 64 * t + 16 * s * kStride;
+        const uintx2 lo = __builtin_bit_cast(uintx2, column_of_4(from));
+        const uintx2 hi = __builtin_bit_cast(uintx2, column_of_4(from + 8 * kStride));
+        v[i] = uintx4{lo[0], lo[1], hi[0], hi[1]};
+      }
+      o[t] = mma_terms(v, w, o[t]);
+    }
+  }
+}
+
 // What weighted_sum<SAFE> left out, for the rows that see it: a weight of a key that is
 // seen is positive, so the sum gets the infinity or NaN itself.  seen: the lane's keys of
 // the tile, valid: those that exist.
@@ -246,8 +343,8 @@ __device__ __forceinline__ void softmax_step(floatx16* s, floatx16* o, Running& 
 
 // The wavefront's partial sums, where the keys are cut into pieces.
 template <int DP>
-__device__ __forceinline__ void store_partial(const AttentionArgs& a, const floatx16* o, const Running& r,
-                                              int token, int head, int piece, int lane) {
+__device__ __forceinline__ void store_partial(const AttentionArgs& a, const floatx16* o, float m, float l, int token,
+                                              int head, int piece, int lane) {
   const long at = (static_cast<long>(piece) * a.total_q + token) * a.heads + head;
   float* to = a.partial + at * DP + 4 * (lane >> 5);
 #pragma unroll
@@ -257,8 +354,8 @@ __device__ __forceinline__ void store_partial(const AttentionArgs& a, const floa
       *reinterpret_cast<floatx4*>(to + 32 * t + 8 * i) =
           floatx4{o[t][4 * i], o[t][4 * i + 1], o[t][4 * i + 2], o[t][4 * i + 3]};
   if (lane < 32) {
-    a.stats[2 * at] = r.m;
-    a.stats[2 * at + 1] = r.l;
+    a.stats[2 * at] = m;
+    a.stats[2 * at + 1] = l;
   }
 }
 
@@ -268,7 +365,7 @@ __device__ __forceinline__ void store_partial(const AttentionArgs& a, const floa
 // Nothing reads them soon, and past the cache they leave its room to the keys (252 -> 238).
 template <typename T, int DP>
 __device__ __forceinline__ void store_out(const AttentionArgs& a, const floatx16* o, float inverse, char* lds,
-                                          int q0, int hk, int first, int rows, int lane) {
+                                          int q0, int hk, int first, int rows, unsigned long keep, int lane) {
   using S = TileShape<T, DP>;
   typedef T vec4 __attribute__((ext_vector_type(4)));
   char* const mine = lds + (lane & 31) * S::kOutStride + 4 * (lane >> 5) * static_cast<int>(sizeof(T));
@@ -288,7 +385,7 @@ __device__ __forceinline__ void store_out(const AttentionArgs& a, const floatx16
 #pragma unroll
     for (int i = 0; i < 32 / S::kRun; ++i) {
       const int r = i * S::kRun + lane / S::kLanes, row = first + r;
-      if (row < rows) {
+      if (row < rows && (keep >> r & 1)) {
         const int token = a.group.quotient(row), head = hk * group + (row - token * group);
         T* out = static_cast<T*>(a.out.data) + (q0 + token) * a.out.token_stride + head * a.out.head_stride;
         __builtin_nontemporal_store(*reinterpret_cast<const floatx4*>(lds + r * S::kOutStride + chunk * 16),
@@ -298,14 +395,14 @@ __device__ __forceinline__ void store_out(const AttentionArgs& a, const floatx16
 }
 
 template <typename T, int DP, Source SRC, int W>
-__global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attention_tile_kernel(
+__global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attention_tile_kernel(
     const AttentionArgs a) {
   using S = TileShape<T, DP, W>;
   constexpr bool PAGED = SRC != Source::kPacked;
   constexpr int KT = S::kKeys, SUB = KT / 32;
   __shared__ __attribute__((aligned(16))) char lds[S::kLds];
-  char* const lds_k = lds;                        // two tiles of keys
-  char* const lds_v = lds + 2 * KT * S::kKStride;  // ... and of values
+  char* const lds_k = lds;                        // tiles of keys
+  char* const lds_v = lds + S::kBuffers * S::kKTile;  // ... and of values
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = a.group.d, D = a.head_dim;
@@ -339,17 +436,28 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
   if (PAGED && piece > 0 && begin >= all) return;
 
   const int* const table = PAGED ? a.block_table + static_cast<long>(seq) * a.table_width : nullptr;
-  // queries: 16 bytes per 16 (fp32: 8) values of d, the lane's half of them
-  floatx4 q[S::kChunks / 2];
-  {
-    const char* at = reinterpret_cast<const char*>(static_cast<const T*>(a.q.data) +
-                                                   (q0 + token) * a.q.token_stride + head * a.q.head_stride);
+  // queries: 16 bytes per 16 (fp32: 8) values of d, the lane's half of them; by terms 8 values
+  // of 16, half of them the lane's
+  floatx4 q[S::kSplit ? 1 : S::kChunks / 2];
+  uintx4 q_terms[S::kSplit ? DP / 16 : 1][3];
+  const char* const q_at = reinterpret_cast<const char*>(static_cast<const T*>(a.q.data) +
+                                                         (q0 + token) * a.q.token_stride + head * a.q.head_stride);
+  const auto q_chunk = [&](int chunk) {
+    return chunk * static_cast<int>(16 / sizeof(T)) < D ? *reinterpret_cast<const floatx4*>(q_at + chunk * 16) : floatx4{};
+  };
+  if constexpr (S::kSplit) {
 #pragma unroll
-    for (int s = 0; s < S::kChunks / 2; ++s) {
-      const int chunk = 2 * s + (lane >> 5);
-      q[s] = floatx4{};
-      if (chunk * static_cast<int>(16 / sizeof(T)) < D) q[s] = *reinterpret_cast<const floatx4*>(at + chunk * 16);
-    }
+    for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const floatx4 x = q_chunk(4 * s + 2 * (lane >> 5) + e);
+        const Terms lo = terms_of(x[0], x[1]), hi = terms_of(x[2], x[3]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) q_terms[s][i][2 * e] = lo.t[i], q_terms[s][i][2 * e + 1] = hi.t[i];
+      }
+  } else {
+#pragma unroll
+    for (int s = 0; s < S::kChunks / 2; ++s) q[s] = q_chunk(2 * s + (lane >> 5));
   }
 
   // Staging.  Chunks past head_dim are zeroed in LDS once and not written again.
@@ -367,17 +475,6 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
   const int run_row = lane / S::kLanes;  // of the rows that the wavefront loads
   const unsigned k_off = (SRC == Source::kRuns ? run_row : pass_row) * static_cast<unsigned>(k_stride) + chunk_at;
   const unsigned v_off = (SRC == Source::kRuns ? run_row : pass_row) * static_cast<unsigned>(v_stride) + chunk_at;
-  char* const put_k = lds_k + pass_row * S::kKStride + chunk * 16;
-  char* const put_v = lds_v + pass_row * S::kVStride + chunk * 16;
-  if (S::kLanes != S::kChunks || DP != D) {
-    if (!there && chunk < S::kChunks)
-#pragma unroll
-      for (int i = 0; i < 2 * S::kStage; ++i) {
-        const int b = i / S::kStage, r = i % S::kStage * S::kPass;
-        *reinterpret_cast<floatx4*>(put_k + b * KT * S::kKStride + r * S::kKStride) = floatx4{};
-        *reinterpret_cast<floatx4*>(put_v + b * KT * S::kVStride + r * S::kVStride) = floatx4{};
-      }
-  }
   floatx4 stage_k[S::kStage], stage_v[S::kStage];
   constexpr unsigned long kAllValid = KT == 64 ? ~0ul : (1ul << KT) - 1;
   // kRuns: 64 entries of the block table, one per lane, from block `window` on, and those 32
@@ -444,15 +541,41 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
       }
     }
   };
-  auto put = [&](int buffer) {
-    if (there)
+  bool strange = false;  // by terms: some value was not finite, and went in as zero
+  auto write = [&](auto safe, int buffer) {
+    constexpr bool TERMS = S::kSplit && !decltype(safe)::value;
+    char* const to_k = lds_k + buffer * S::kKTile;
+    char* const to_v = lds_v + buffer * S::kVTile;
+    if constexpr (TERMS) {
+#pragma unroll
+      for (int i = 0; i < S::kStage; ++i)
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          floatx4 x = kv ? stage_v[i] : stage_k[i];
+          if (kv)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool finite = __builtin_isfinite(x[e]);
+              strange |= !finite;
+              x[e] = finite ? x[e] : 0.f;
+            }
+          const Terms lo = terms_of(x[0], x[1]), hi = terms_of(x[2], x[3]);
+          constexpr int kPlane[2] = {S::kKPlane, S::kVPlane};
+          char* to = (kv ? to_v : to_k) + (pass_row + i * S::kPass) * (kPlane[kv] / KT) + chunk * 8;
+#pragma unroll
+          for (int t = 0; t < 3; ++t) *reinterpret_cast<uintx2*>(to + t * kPlane[kv]) = uintx2{lo.t[t], hi.t[t]};
+        }
+    } else {
 #pragma unroll
       for (int i = 0; i < S::kStage; ++i) {
-        *reinterpret_cast<floatx4*>(put_k + buffer * (KT * S::kKStride) + i * S::kPass * S::kKStride) = stage_k[i];
-        *reinterpret_cast<floatx4*>(put_v + buffer * (KT * S::kVStride) + i * S::kPass * S::kVStride) = stage_v[i];
+        *reinterpret_cast<floatx4*>(to_k + (pass_row + i * S::kPass) * S::kKStride + chunk * 16) = stage_k[i];
+        *reinterpret_cast<floatx4*>(to_v + (pass_row + i * S::kPass) * S::kVStride + chunk * 16) = stage_v[i];
       }
+    }
   };
-
+  auto put = [&](auto safe, int buffer) {
+    if (there) write(safe, buffer);
+  };
   open_window(begin);
   // Blocks that do not exist are looked for once; where there is one, every tile asks for its keys.
   bool missing = false;
@@ -469,6 +592,7 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
   // SAFE: what V's infinities and NaN do to a row is decided by what the row sees.
   auto pass = [&](auto safe) {
     constexpr bool SAFE = decltype(safe)::value;
+    floatx4 q_safe[SAFE && S::kSplit ? S::kChunks / 2 : 1];
 #pragma unroll
     for (int t = 0; t < DP / 32; ++t) o[t] = floatx16{};
     run = Running();
@@ -477,18 +601,31 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
       open_window(begin);
       fetch(begin);
     }
-    put(0);
+    if constexpr (SAFE && S::kSplit) {
+#pragma unroll
+      for (int s = 0; s < S::kChunks / 2; ++s) q_safe[s] = q_chunk(2 * s + (lane >> 5));
+    }
+    if (!there && chunk < S::kChunks) {  // chunks past head_dim: zero once
+#pragma unroll
+      for (int i = 0; i < S::kStage; ++i) stage_k[i] = stage_v[i] = floatx4{};
+      for (int b = 0; b < S::kBuffers; ++b) write(safe, b);
+    }
+    put(safe, 0);
     if (begin + KT < end) fetch(begin + KT);
     __syncthreads();
     int buffer = 0;
     for (int at = begin; at < end; at += KT) {
       const bool work = at < high;
-      const char* const now_k = lds_k + buffer * (KT * S::kKStride);
-      const char* const now_v = lds_v + buffer * (KT * S::kVStride);
+      const char* const now_k = lds_k + buffer * S::kKTile;
+      const char* const now_v = lds_v + buffer * S::kVTile;
       floatx16 s[SUB];
-      if (work) scores<T, DP>(now_k, q, s, lane);
-      if (at + KT < end) {
-        put(buffer ^ 1);
+      if (work) {
+        if constexpr (!S::kSplit) scores<T, DP>(now_k, q, s, lane);
+        else if constexpr (SAFE) scores<T, DP>(now_k, q_safe, s, lane);
+        else scores_by_terms<DP>(now_k, q_terms, s, lane);
+      }
+      if (S::kBuffers == 2 && at + KT < end) {
+        put(safe, buffer ^ 1);
         if (at + 2 * KT < end) fetch(at + 2 * KT);
       }
       if (work) {
@@ -506,32 +643,57 @@ __global__ __launch_bounds__(64 * W, DP * sizeof(T) <= 256 ? 2 : 1) void attenti
             }
         }
         softmax_step<T, DP, SUB>(s, o, run, a.scale_log2);
-        weighted_sum<T, DP, SAFE>(now_v, s, o, lane);
+        if constexpr (S::kSplit && !SAFE) weighted_sum_by_terms<DP>(now_v, s[0], o, lane);
+        else weighted_sum<T, DP, SAFE>(now_v, s, o, lane);
         if (SAFE) add_not_finite<T, DP>(now_v, min(min(limit, end) - at, KT), valid, o, lane);
       }
-      buffer ^= 1;
       __syncthreads();
+      if constexpr (S::kBuffers == 2) {
+        buffer ^= 1;
+      } else if (at + KT < end) {
+        put(safe, 0);
+        if (at + 2 * KT < end) fetch(at + 2 * KT);
+        __syncthreads();
+      }
     }
   };
+  // The rows of `keep`: out and lse, or their partial sums.
+  const auto finish = [&](bool keep) {
+    const float l = run.l + __shfl_xor(run.l, 32, 64);
+    if (PAGED && all > a.piece) {
+      if (real && keep) store_partial<DP>(a, o, run.m, l, q0 + token, head, piece, lane);
+      return;
+    }
+    store_out<T, DP>(a, o, l == 0.f ? 0.f : 1.f / l, lds + wave * (32 * S::kOutStride), q0, hk, first + 32 * wave,
+                     rows, __ballot(keep), lane);
+    if (a.lse && real && keep && lane < 32)
+      a.lse[static_cast<long>(head) * a.total_q + q0 + token] =
+          l == 0.f ? -INFINITY : (run.m - kLift<T> + log2f(l)) * 0.69314718f;
+  };
+  const auto finite = [&] {
+    float check = 0.f;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) check += 0.f * o[t][i];
+    return check + __shfl_xor(check, 32, 64) == 0.f;  // (0 * inf and 0 * NaN are NaN)
+  };
   pass(std::false_type());
-  // A weight of zero does not keep an infinity or NaN in V's row out of the products.  If
-  // some row's sums are not finite, everything is done once more, the safe way.
-  float check = 0.f;
-#pragma unroll
-  for (int t = 0; t < DP / 32; ++t)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) check += 0.f * o[t][i];
-  if (__syncthreads_or(check != 0.f)) pass(std::true_type());  // (0 * inf and 0 * NaN are NaN, which is not 0)
-  run.l += __shfl_xor(run.l, 32, 64);
-  if (PAGED && all > a.piece) {
-    if (real) store_partial<DP>(a, o, run, q0 + token, head, piece, lane);
-    return;
+  // A weight of zero does not keep an infinity or NaN in V's row out of the products, and terms
+  // make NaN of infinities.  If some row's sums are not finite, everything is done once more,
+  // the safe way.  By terms that way is another (products of fp32), and rows that do not need
+  // it keep their first result: what others hold does not change a row's bits.
+  const bool good = finite();
+  bool keep = true;
+  if (__syncthreads_or(!good || strange)) {
+    if constexpr (S::kSplit) {
+      finish(good);
+      __syncthreads();
+    }
+    pass(std::true_type());
+    if constexpr (S::kSplit) keep = !good || !finite();
   }
-  store_out<T, DP>(a, o, run.l == 0.f ? 0.f : 1.f / run.l, lds + wave * (32 * S::kOutStride), q0, hk,
-                   first + 32 * wave, rows, lane);
-  if (a.lse && real && lane < 32)
-    a.lse[static_cast<long>(head) * a.total_q + q0 + token] =
-        run.l == 0.f ? -INFINITY : (run.m - kLift<T> + log2f(run.l)) * 0.69314718f;
+  finish(keep);
 }
 
 }  // namespace mchip
