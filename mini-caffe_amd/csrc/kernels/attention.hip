@@ -4,6 +4,8 @@
 //   m' = max(m, s), l' = l e^(m - m') + sum e^(s - m'), o' = o e^(m - m') + sum e^(s - m') v.
 #include "attention_args.h"
 
+#include <algorithm>
+#include <climits>
 #include <cmath>
 
 namespace mchip {
@@ -93,7 +95,9 @@ extern "C" int mcAttentionPaged(const mcAttentionGeom* geom, const mcHeads* q, c
   a.num = num_requests;
   a.total_q = total_q;
   a.max_q = max_q;
-  a.max_context = max_context;
+  // no more than the table holds, and room for the kernels' rounding up to tiles
+  a.max_context = static_cast<int>(std::min({static_cast<long>(max_context), static_cast<long>(table_width) * cache->block_size,
+                                             static_cast<long>(INT_MAX) - 65535}));
   a.lse = lse;
   return launch(a, geom->type, true, static_cast<hipStream_t>(stream));
 }

@@ -46,17 +46,6 @@ struct AttentionArgs {
   int* counters;   // attention_rows.h: [num * heads_kv], zero
 };
 
-// The last sequence that starts at row `at` of the packed queries or before it.
-__device__ __forceinline__ int sequence_of_row(const int* __restrict__ starts, int num, int at) {
-  int lo = 0, hi = num;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= at) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
 // A tile of query rows, found by a whole wavefront (the same in every wavefront).
 struct TileId {
   int seq;
@@ -66,13 +55,14 @@ struct TileId {
 };
 
 // Tile number `slot` of one key head: sequence s's tiles begin at slot starts[s] * group /
-// rows + s (s leaves room for the ragged ends).  All that describes up to 64 sequences is
+// rows + s * gap (gap 1 leaves room for the ragged ends; with group = rows = 1 and gap 0 a slot
+// is a row of the packed queries).  All that describes up to 64 sequences is
 // loaded at once, a sequence per lane; a bisection in memory would wait for one load after
 // another.
 template <bool PAGED>
-__device__ __forceinline__ TileId find_tile(const AttentionArgs& a, int slot, int rows_per_tile) {
-  const int lane = threadIdx.x & 63, group = a.group.d;
-  const auto starts_at = [&](int s) { return static_cast<long>(a.q_starts[s]) * group / rows_per_tile + s; };
+__device__ __forceinline__ TileId find_tile(const AttentionArgs& a, int slot, int group, int rows_per_tile, int gap) {
+  const int lane = threadIdx.x & 63;
+  const auto starts_at = [&](int s) { return static_cast<long>(a.q_starts[s]) * group / rows_per_tile + s * gap; };
   int lo = 0, n = a.num;
   while (n > 64) {
     const int step = (n + 63) / 64, s = lo + lane * step;
@@ -87,7 +77,7 @@ __device__ __forceinline__ TileId find_tile(const AttentionArgs& a, int slot, in
   t.q1 = min(a.q_starts[s + 1], a.total_q);
   t.k0 = PAGED ? 0 : a.k_starts[s];
   t.k1 = PAGED ? a.context_lens[s] : a.k_starts[s + 1];
-  const long at = static_cast<long>(raw) * group / rows_per_tile + s;
+  const long at = static_cast<long>(raw) * group / rows_per_tile + s * gap;
   const int chosen = max(__popcll(__ballot(lane < n && at <= slot)) - 1, 0);
   t.seq = lo + chosen;
   t.index = __builtin_amdgcn_readlane(static_cast<int>(slot - at), chosen);

@@ -11,43 +11,65 @@
 namespace mchip {
 namespace {
 
-// Rows whose keys were cut into pieces: the pieces' sums, weighted by e^(m_piece - m).  One
-// wavefront per row and head.
+constexpr int kMostPieces = 64;  // a lane holds the statistics of one
+
+// Rows whose keys were cut into pieces: the pieces' sums, weighted by 2^(m_piece - m).  One
+// wavefront per row and head, which asks for all it needs in three steps: the sequences'
+// bounds, the pieces' statistics (a lane each), their sums.
 template <typename T, int DP>
 __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs a) {
+  constexpr int kPer = DP <= 64 ? 1 : DP <= 128 ? 2 : 4;  // contiguous values of a lane
   const long at = blockIdx.x * 4l + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (at >= static_cast<long>(a.total_q) * a.heads) return;
-  const int token = static_cast<int>(at / a.heads), head = static_cast<int>(at - static_cast<long>(token) * a.heads);
-  const int seq = sequence_of_row(a.q_starts, a.num, token);
-  const int q0 = max(a.q_starts[seq], 0), q1 = min(a.q_starts[seq + 1], a.total_q);
-  const int queries = min(q1 - q0, a.max_q);
+  const int token = __builtin_amdgcn_readfirstlane(static_cast<int>(at / a.heads));
+  const int head = __builtin_amdgcn_readfirstlane(static_cast<int>(at - static_cast<long>(token) * a.heads));
+  const TileId tile = find_tile<true>(a, token, 1, 1, 0);
+  const int q0 = __builtin_amdgcn_readfirstlane(tile.q0), q1 = __builtin_amdgcn_readfirstlane(tile.q1);
+  const int queries = min(q1 - q0, a.max_q), group = a.group.d;
   if (token < q0 || token - q0 >= queries) return;
-  const int all = keys_of_tile<true>(a, keys_of<true>(a, 0, a.context_lens[seq], q1 - q0), (token - q0) * static_cast<int>(a.group.d) +
-                                     head % static_cast<int>(a.group.d), queries * static_cast<int>(a.group.d), a.tile_rows);
+  const Keys keys = keys_of<true>(a, 0, __builtin_amdgcn_readfirstlane(tile.k1), q1 - q0);
+  const int all = keys_of_tile<true>(a, keys, (token - q0) * group + head % group, queries * group, a.tile_rows);
   if (all <= a.piece) return;  // written by the one workgroup that had all of its keys
   const int pieces = (all + a.piece - 1) / a.piece;
   const long step = static_cast<long>(a.total_q) * a.heads;
-  float m = -INFINITY;
-  for (int p = 0; p < pieces; ++p) m = fmaxf(m, a.stats[2 * (p * step + at)]);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o[(DP + 63) / 64] = {};
-  for (int p = 0; p < pieces; ++p) {
-    const long from = p * step + at;
-    const float w = exp2f(a.stats[2 * from] - base);
-    l += w * a.stats[2 * from + 1];
+  float m = -INFINITY, l = 0.f;
+  if (lane < pieces) {
+    const floatx2 stat = *reinterpret_cast<const floatx2*>(a.stats + 2 * (lane * step + at));
+    m = stat[0];
+    l = stat[1];
+  }
+  float top = m;
 #pragma unroll
-    for (int i = 0; i < (DP + 63) / 64; ++i)
-      if (lane + 64 * i < DP) o[i] += w * a.partial[from * DP + lane + 64 * i];
+  for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w, 64));
+  const float weight = exp2f(m - (top == -INFINITY ? 0.f : top));
+  l *= weight;
+#pragma unroll
+  for (int w = 32; w > 0; w >>= 1) l += __shfl_xor(l, w, 64);
+  typedef float vecf __attribute__((ext_vector_type(kPer)));
+  typedef T vec __attribute__((ext_vector_type(kPer)));
+  vecf o = {};
+  const int d = min(lane * kPer, DP - kPer);
+  const float* from = a.partial + at * DP + d;
+  constexpr int kAhead = 8;
+  for (int p0 = 0; p0 < pieces; p0 += kAhead) {
+    vecf x[kAhead];
+#pragma unroll
+    for (int p = 0; p < kAhead; ++p) x[p] = *reinterpret_cast<const vecf*>(from + min(p0 + p, pieces - 1) * step * DP);
+#pragma unroll
+    for (int p = 0; p < kAhead; ++p)
+      if (p0 + p < pieces) o += __shfl(weight, p0 + p, 64) * x[p];
   }
   const float inverse = l == 0.f ? 0.f : 1.f / l;
-  T* out = static_cast<T*>(a.out.data) + token * a.out.token_stride + head * a.out.head_stride;
+  if (lane * kPer < a.head_dim) {
+    vec y;
 #pragma unroll
-  for (int i = 0; i < (DP + 63) / 64; ++i)
-    if (lane + 64 * i < a.head_dim) out[lane + 64 * i] = static_cast<T>(o[i] * inverse);
+    for (int e = 0; e < kPer; ++e) y[e] = static_cast<T>(o[e] * inverse);
+    *reinterpret_cast<vec*>(static_cast<T*>(a.out.data) + token * a.out.token_stride + head * a.out.head_stride + d) = y;
+  }
   if (a.lse && lane == 0)
     a.lse[static_cast<long>(head) * a.total_q + token] =
-        l == 0.f ? -INFINITY : (m - kLift<T> + log2f(l)) * 0.69314718f;
+        l == 0.f ? -INFINITY : (top - kLift<T> + log2f(l)) * 0.69314718f;
 }
 
 template <typename T, int DP, bool PAGED, int W>
@@ -59,17 +81,22 @@ int launch_tiles(AttentionArgs a, hipStream_t st) {
   a.pieces = 1;
   a.piece = a.max_context;
   if (PAGED) {
-    // Too few tiles to fill the GPU: cut the keys, into the number of pieces whose rounds of
-    // workgroups, each a piece and about five tiles' time to begin and end, take least.  (A
-    // chunk of 512 over 32768, 32/8 heads of 128 in bf16, eight wavefronts: two pieces 537 us,
-    // three 369, four, which give every CU one workgroup, 309, six 395, eight 324.)
-    const long tiles = std::max<long>(ceil_div(a.total_q * group, S::kRows), std::min(a.num, a.total_q));
-    const long items = tiles * a.heads_kv, slots = 8 / W * kNumCu;
-    const int most = std::max(1, std::min(a.max_context / (4 * S::kKeys), 64));
+    // Too few tiles to fill the GPU: cut the keys, into the number of pieces that takes least
+    // time, counted in keys: rounds of workgroups, each a piece and about five tiles' time to
+    // begin and end, and the pieces' sums written and read (4 bytes a ps, and a key takes 32 ns: 128 kB).
+    // A chunk of 512 over 32768, 32/8 heads of 128 in bf16, eight wavefronts: two pieces 556 us,
+    // three 381, four, which give every CU one workgroup, 314, six 400, eight 328.  48 chunks of
+    // up to 202 over up to 1685, 16/1 heads: one piece 111, two 144.  How many tiles there are
+    // the GPU knows; about half a tile per sequence is not full.
+    const long tiles = a.num == 1 ? ceil_div(a.total_q * group, S::kRows)
+                                  : std::max<long>(a.total_q * group / S::kRows + (a.num + 1) / 2, std::min(a.num, a.total_q));
+    const long items = tiles * a.heads_kv, slots = (W == 8 || DP > 128 ? 1 : 2) * kNumCu;
+    const long sums = static_cast<long>(a.total_q) * a.heads * DP * 8;  // bytes of one piece, both ways
+    const int most = std::max(1, std::min(a.max_context / (4 * S::kKeys), kMostPieces));
     int wanted = 1;
     long best = LONG_MAX;
     for (int p = 1; p <= most && (p == 1 || items * (p - 1) < 2 * slots); ++p) {
-      const long time = (items * p + slots - 1) / slots * (ceil_div(a.max_context, p) + 5 * S::kKeys);
+      const long time = (items * p + slots - 1) / slots * (ceil_div(a.max_context, p) + 5 * S::kKeys) + (p > 1 ? p * sums / 128000 : 0);
       if (time < best) best = time, wanted = p;
     }
     a.piece = std::max(ceil_div(ceil_div(a.max_context, wanted), S::kKeys), 1) * S::kKeys;
@@ -149,7 +176,9 @@ int launch_rows(const AttentionArgs& a, hipStream_t st) {
   // 12 heads 191 and 172; three of 100 to 300 39 and 43.  (64 values: 4096 twice, 12 heads, not
   // causal, 548 and 588.)
   if constexpr (sizeof(T) == 4 && DP > 64 && DP <= 128)
-    if (rows / a.num >= 512 && keys >= 512) return launch_tiles<T, DP, PAGED, 8>(a, st);
+    if (rows / a.num >= 512 && keys >= 512 &&
+        (PAGED || rows * a.heads_kv >= 1l * kNumCu * TileShape<T, DP, 8>::kRows))
+      return launch_tiles<T, DP, PAGED, 8>(a, st);
   return launch_tiles<T, DP, PAGED, 4>(a, st);
 }
 

@@ -412,7 +412,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attention_tile_kern
   const int rest = blockIdx.x / a.heads_kv;
   const int piece = PAGED ? rest / a.tiles : 0;
   // Tiles run from the last, which sees most keys of a causal sequence, to the first.
-  const TileId tile = find_tile<PAGED>(a, a.tiles - 1 - (rest - piece * a.tiles), S::kRows);
+  const TileId tile = find_tile<PAGED>(a, a.tiles - 1 - (rest - piece * a.tiles), group, S::kRows, 1);
   // (said to be scalars, or the loop bounds below are vectors)
   const int seq = __builtin_amdgcn_readfirstlane(tile.seq);
   const int q0 = __builtin_amdgcn_readfirstlane(tile.q0), q1 = __builtin_amdgcn_readfirstlane(tile.q1);

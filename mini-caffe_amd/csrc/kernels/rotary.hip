@@ -23,7 +23,7 @@ struct RotaryArgs {
   mcHeads q, q_out, k, k_out, v;  // data null: not there
   mcPagedCache cache;             // keys null: none
   const int* slots;
-  unsigned char axis[kMaxPairs];
+  unsigned axis[kMaxPairs / 16];  // two bits a pair (launch arguments cost the host 2 ns a byte)
 };
 
 template <typename T, int N>
@@ -82,9 +82,10 @@ template <typename T, int N, bool ADJACENT>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
   __shared__ float cs[kMaxPairs], sn[kMaxPairs];
   const int t = blockIdx.x, tid = threadIdx.x;
-  if (tid < a.pairs)
-    sincosf(static_cast<float>(a.positions[a.axis[tid] * a.axis_stride + t]) * a.frequencies[tid], &sn[tid],
-            &cs[tid]);
+  if (tid < a.pairs) {
+    const int axis = a.axis[tid >> 4] >> 2 * (tid & 15) & 3;
+    sincosf(static_cast<float>(a.positions[axis * a.axis_stride + t]) * a.frequencies[tid], &sn[tid], &cs[tid]);
+  }
   __syncthreads();
   long cache_row = -1;
   if (a.cache.keys) {
@@ -163,11 +164,12 @@ extern "C" int mcRotary(const mcRotaryGeom* geom, const float* frequencies, cons
   MC_REQUIRE(sum == a.pairs, "%s: the sections hold %d pairs of %d", who, sum, a.pairs);
   for (int i = 0, axis = 0; i < a.pairs; ++i) {
     while (left[axis] == 0) axis = (axis + 1) % geom->num_axes;
-    a.axis[i] = static_cast<unsigned char>(axis);
+    a.axis[i >> 4] |= static_cast<unsigned>(axis) << 2 * (i & 15);
     --left[axis];
     if (geom->cycled) axis = (axis + 1) % geom->num_axes;
   }
   MC_REQUIRE(tokens >= 0, "%s: %d tokens", who, tokens);
+  MC_REQUIRE(axis_stride >= 0, "%s: axis_stride %ld is negative", who, axis_stride);
   if (tokens == 0) return 0;
   MC_REQUIRE(frequencies && positions, "%s: null argument", who);
   if (check_heads(who, "q", q, geom->type) || check_heads(who, "q_out", q_out, geom->type)) return -1;
