@@ -1,5 +1,5 @@
-// Attention of many query rows: a workgroup of four wavefronts holds a tile of rows in
-// registers and passes over the keys, a tile at a time through LDS.
+// Attention of many query rows: a workgroup of four or eight wavefronts holds a tile of rows
+// in registers and passes over the keys, a tile at a time through LDS.
 //
 // Rows: the query heads of one key head lie behind each other (row = token * group + head
 // of the group), so a tile reads the keys of its one key head, whatever the group.  A
@@ -17,9 +17,10 @@
 // (ds_read_b64_tr_b16: of 16 lanes that address 4 rows of 16 values, each gets a column).
 //
 // fp32 rows of at most 128 values: each value is the sum of three bf16, x = h + m + l exact to
-// its last bit, and a product the six of them that reach 2^-24 of it (h h', h m', m h', m m',
-// h l', l h'; what is left out, m l' and l m', is below 2^-23 each and 2^-26 on the whole), on the matrix unit's bf16 rate, sixteen times
-// that of fp32.  The terms are formed on the way into LDS, once per workgroup.
+// its last bit, and a product is six of theirs (h h', h m', m h', m m', h l', l h'; what is left
+// out, m l' and l m', is below 2^-23 of it and on the whole near 2^-26), at the matrix unit's
+// bf16 rate, sixteen times that of fp32.  The terms are formed on the way into LDS, once per
+// workgroup.
 #ifndef MCHIP_ATTENTION_TILE_H_
 #define MCHIP_ATTENTION_TILE_H_
 
@@ -34,12 +35,10 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 typedef short shortx8 __attribute__((ext_vector_type(8)));
 
-// What differs by element type: the operand registers and the products.
+// A product of 16 values of d, or of keys, in fp16 or bf16: a lane supplies eight.
 template <typename T>
-struct Product {  // fp16, bf16
+struct Product {
   typedef T vec8 __attribute__((ext_vector_type(8)));
-  typedef vec8 Operand;               // 8 values of d, or of keys: 16 per product
-  static constexpr int kDepth = 16;
   static __device__ __forceinline__ floatx16 mma(vec8 a, vec8 b, floatx16 c) {
     if constexpr (__is_same(T, bf16_t)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     else return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
@@ -302,10 +301,12 @@ struct Running {
   float m = -INFINITY, l = 0.f;
 };
 
-// The weights of fp16 are kept this many powers of two larger than those of the largest
-// score, so that small ones stay out of fp16's subnormal range.
+// The weights are kept this many powers of two away from 1 for the largest score: in fp16
+// above, so that small ones stay out of its subnormal range; in the others, whose range is
+// fp32's, below, so that sums of values near the largest there are do not overflow before they
+// are divided.
 template <typename T>
-constexpr float kLift = __is_same(T, half_t) ? 10.f : 0.f;
+constexpr float kLift = __is_same(T, half_t) ? 10.f : -16.f;
 // m moves only when a score is this much above it (in powers of two): the sums are then
 // rescaled for a few tiles of a pass instead of most, and weights reach 2^8 (fp16: 2^15,
 // just within its range).  The quotient at the end does not depend on m.
@@ -427,9 +428,9 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attention_tile_kern
   const bool real = first + 32 * wave + (lane & 31) < rows;
   const int token = a.group.quotient(row), head = hk * group + (row - token * group);
   const int limit = max(min(keys.count, a.causal ? keys.offset + token : keys.count), 0);
-  // rows see more from the first to the last of a wavefront
+  // rows see more from the first to the last of a wavefront (one without rows of its own: nothing)
   const int low = __builtin_amdgcn_readfirstlane(limit);
-  const int high = __builtin_amdgcn_readlane(limit, 31);
+  const int high = first + 32 * wave < rows ? __builtin_amdgcn_readlane(limit, 31) : 0;
   const int all = keys_of_tile<PAGED>(a, keys, first, rows, S::kRows);  // over the workgroup's
   const int begin = PAGED ? min(piece * a.piece, all) : 0;
   const int end = PAGED ? static_cast<int>(min(static_cast<long>(begin) + a.piece, static_cast<long>(all))) : all;

@@ -496,3 +496,83 @@ def test_refusals_paged(A):
     call(max_q=0)
     with pytest.raises(ValueError):
         A.PagedCache.of(c, c[:2])
+
+
+# ---- many sequences, and values at the ends of the range ---------------------------------
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("count", [64, 65, 200, 4200])
+def test_packed_many_sequences(A, kind, count):
+    """Finding a row tile's sequence among more than a wavefront's lanes; empty sequences among them."""
+    g = torch.Generator(device="cuda").manual_seed(22)
+    lengths = [(7 * i) % 4 if count > 1000 else (13 * i) % 37 for i in range(count)]
+    n = sum(lengths)
+    q, k, v = (randn(g, n, h, 64, kind=kind) for h in (2, 1, 1))
+    out, lse = packed(A, q, k, v, lengths, lengths, True)
+    check_packed(q, k, v, lengths, lengths, True, out, lse)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("count,longest", [(70, 3), (130, 40)])
+def test_paged_many_requests(A, kind, count, longest):
+    """Chunks of many requests, some empty, over contexts long enough to be cut into pieces."""
+    g = torch.Generator(device="cuda").manual_seed(23)
+    q_lens = [(11 * i) % (longest + 1) for i in range(count)]
+    contexts = [n + (29 * i) % 60 + (900 if i == 3 else 0) for i, n in enumerate(q_lens)]
+    keys, values, table, ks, vs = make_cache(g, contexts, 16, 1, 64, kind)
+    q = randn(g, sum(q_lens), 2, 64, kind=kind)
+    out, lse = paged(A, q, keys, values, table, q_lens, contexts)
+    check_paged(q, ks, vs, q_lens, contexts, out, lse)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 200])
+@pytest.mark.parametrize("sizes", [(1e18, 1e-18, 1.0), (1e-18, 1e18, 1.0), (1.0, 1.0, 1e37), (1.0, 1.0, 1e-30), (1e-20, 1e-10, 1.0)])
+def test_packed_fp32_over_its_range(A, dim, sizes):
+    """Values far from one, whose terms in fewer bits have to reach as far as fp32 does."""
+    g = torch.Generator(device="cuda").manual_seed(24)
+    q, k, v = (randn(g, 150, 1, dim) * s for s in sizes)
+    out, lse = packed(A, q, k, v, [150], [150], True)
+    check_packed(q, k, v, [150], [150], True, out, lse)
+
+
+def test_packed_fp32_largest_values(A):
+    """Finite values that round to infinity in bf16 stay finite."""
+    g = torch.Generator(device="cuda").manual_seed(25)
+    q, k, v = (randn(g, 100, 1, 64) for _ in range(3))
+    v[::2] = torch.finfo(torch.float32).max
+    v[1::2] = -torch.finfo(torch.float32).max
+    v /= 4
+    v[5] = torch.finfo(torch.float32).max
+    q[:, :, 0], k[:, :, 0] = 3.4e38, 0.0
+    out, lse = packed(A, q, k, v, [100], [100], True)
+    # the sum of weights times values stays within 1.25 / 4 of the largest but in row 5 and those that weigh it
+    assert torch.isfinite(lse).all()
+    rows = [r for r in range(5)]
+    check_packed(q[rows], k[rows], v[rows], [5], [5], True, out[rows], lse[:, rows])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("where", ["packed", "single", "chunk"])
+def test_infinite_keys(A, kind, where):
+    """A key of infinity gives scores of plus and minus infinity: rows with the first are NaN, the others ignore it."""
+    g = torch.Generator(device="cuda").manual_seed(26)
+    n, d, at = 60, 64, 20
+    q_len = {"packed": n, "single": 1, "chunk": 40}[where]
+    q, k, v = randn(g, q_len, 1, d, kind=kind), randn(g, n, 1, d, kind=kind), randn(g, n, 1, d, kind=kind)
+    k[at] = 0
+    k[at, 0, 7] = float("inf")
+    if where == "packed":
+        out, _ = packed(A, q, k, v, [n], [n], True)
+    else:
+        keys, values = (torch.zeros((4, 16, 1, d), dtype=TYPES[kind], device="cuda") for _ in range(2))
+        keys.view(-1, 1, d)[:n], values.view(-1, 1, d)[:n] = k, v
+        out, _ = paged(A, q, keys, values, ints([0, 1, 2, 3])[None].contiguous(), [q_len], [n])
+    for r in range(q_len):
+        sees = n - q_len + r + 1
+        if sees > at and q[r, 0, 7] > 0:
+            assert torch.isnan(out[r]).all()
+        else:
+            kept = [j for j in range(sees) if j != at]
+            want = rows64(q[r:r + 1, 0], k[kept, 0], v[kept, 0], 1 / 8, [len(kept)])
+            lse = torch.log(torch.exp(torch.zeros(1))) + want[1]
+            check(kind, d, n, out[r:r + 1, 0], lse, want, 5.0)
