@@ -578,7 +578,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attention_tile_kern
     if (there) write(safe, buffer);
   };
   open_window(begin);
-  // Blocks that do not exist are looked for once; where there is one, every tile asks for its keys.
+  // Blocks that do not exist are looked for once; where there is one, the safe pass leaves them out.
   bool missing = false;
   if (PAGED && begin < end) {
     const int last = a.block.quotient(end - 1);
@@ -590,7 +590,8 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attention_tile_kern
 
   floatx16 o[DP / 32];
   Running run;
-  // SAFE: what V's infinities and NaN do to a row is decided by what the row sees.
+  // SAFE: what V's infinities and NaN do to a row is decided by what the row sees, and keys
+  // without a block are not seen.
   auto pass = [&](auto safe) {
     constexpr bool SAFE = decltype(safe)::value;
     floatx4 q_safe[SAFE && S::kSplit ? S::kChunks / 2 : 1];
@@ -630,17 +631,17 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attention_tile_kern
         if (at + 2 * KT < end) fetch(at + 2 * KT);
       }
       if (work) {
-        const bool masked = at + KT > low || (PAGED && missing);
+        const bool masked = at + KT > low || (SAFE && PAGED && missing);
         unsigned long valid = kAllValid;
         if (masked) {
-          if (PAGED && missing) valid = exist(at);
+          if (SAFE && PAGED && missing) valid = exist(at);
           const int seen = min(limit, end) - at;
 #pragma unroll
           for (int u = 0; u < SUB; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int key = 32 * u + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3);
-              if (key >= seen || (PAGED && !(valid >> key & 1))) s[u][i] = -INFINITY;
+              if (key >= seen || (SAFE && PAGED && !(valid >> key & 1))) s[u][i] = -INFINITY;
             }
         }
         softmax_step<T, DP, SUB>(s, o, run, a.scale_log2);
@@ -679,12 +680,12 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attention_tile_kern
       for (int i = 0; i < 16; ++i) check += 0.f * o[t][i];
     return check + __shfl_xor(check, 32, 64) == 0.f;  // (0 * inf and 0 * NaN are NaN)
   };
-  pass(std::false_type());
+  if (!missing) pass(std::false_type());
   // A weight of zero does not keep an infinity or NaN in V's row out of the products, and terms
   // make NaN of infinities.  If some row's sums are not finite, everything is done once more,
   // the safe way.  By terms that way is another (products of fp32), and rows that do not need
   // it keep their first result: what others hold does not change a row's bits.
-  const bool good = finite();
+  const bool good = !missing && finite();
   bool keep = true;
   if (__syncthreads_or(!good || strange)) {
     if constexpr (S::kSplit) {
