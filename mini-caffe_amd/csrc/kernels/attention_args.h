@@ -6,24 +6,6 @@
 
 namespace mchip {
 
-// n / d for 0 <= n < 2^32 by a product: the round-up method for invariant divisors
-// (Granlund and Montgomery, 1994).
-struct FastDivision {
-  unsigned d, factor;
-  int shift;
-  void set(unsigned divisor) {
-    d = divisor;
-    int log = 0;
-    while ((1ull << log) < divisor) ++log;  // ceil(log2 d)
-    factor = static_cast<unsigned>((((1ull << log) - divisor) << 32) / divisor + 1);
-    shift = log;
-  }
-  __device__ __forceinline__ unsigned quotient(unsigned n) const {
-    const unsigned t = __umulhi(factor, n);
-    return shift == 0 ? n : (t + ((n - t) >> 1)) >> (shift - 1);
-  }
-};
-
 struct AttentionArgs {
   int heads, heads_kv, head_dim, causal;
   FastDivision group;  // query heads of a key head

@@ -4,10 +4,9 @@
 // (rounded to 32 bits): (a, b) -> (a cos - b sin, b cos + a sin).  All heads of a token turn
 // by the same angles, so a workgroup forms a token's cosines and sines once, in LDS, and
 // then passes over its query, key and value heads.  Every value is read and written once:
-// the bound is HBM.
+// the bound is HBM (16384 tokens of 32/8 heads of 128 in bf16, keys and values into the cache:
+// 403 MB in 82 us, 4.9 TB/s, where a large copy reaches 5.2).
 #include "rows_of_heads.h"
-
-#include <algorithm>
 
 namespace mchip {
 namespace {
@@ -23,6 +22,7 @@ struct RotaryArgs {
   mcHeads q, q_out, k, k_out, v;  // data null: not there
   mcPagedCache cache;             // keys null: none
   const int* slots;
+  FastDivision chunks, value_chunks, by_heads, by_heads_kv;  // of a head; heads of a token
   unsigned axis[kMaxPairs / 16];  // two bits a pair (launch arguments cost the host 2 ns a byte)
 };
 
@@ -77,53 +77,76 @@ __device__ __forceinline__ void head_chunk(const T* src, T* dst, T* dst2, int c,
   }
 }
 
-// A workgroup per token.  N: pairs of a chunk, a divisor of `pairs`.
-template <typename T, int N, bool ADJACENT>
-__global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs a) {
-  __shared__ float cs[kMaxPairs], sn[kMaxPairs];
-  const int t = blockIdx.x, tid = threadIdx.x;
-  if (tid < a.pairs) {
-    const int axis = a.axis[tid >> 4] >> 2 * (tid & 15) & 3;
-    sincosf(static_cast<float>(a.positions[axis * a.axis_stride + t]) * a.frequencies[tid], &sn[tid], &cs[tid]);
+// A workgroup takes TB tokens.  N: pairs of a chunk, a divisor of `pairs`.
+template <typename T, int N, bool ADJACENT, int TB>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(const RotaryArgs a) {
+  __shared__ float cs[TB][kMaxPairs], sn[TB][kMaxPairs];
+  __shared__ long cache_rows[TB];
+  const int t0 = blockIdx.x * TB, tid = threadIdx.x, tokens = min(TB, a.tokens - t0);
+  for (int i = tid; i < tokens * kMaxPairs; i += kThreads) {
+    const int t = i / kMaxPairs, p = i % kMaxPairs;
+    if (p < a.pairs) {
+      const int axis = a.axis[p >> 4] >> 2 * (p & 15) & 3;
+      sincosf(static_cast<float>(a.positions[axis * a.axis_stride + t0 + t]) * a.frequencies[p], &sn[t][p], &cs[t][p]);
+    }
+  }
+  if (a.cache.keys && tid < tokens) {
+    const int s = a.slots[t0 + tid];
+    long row = -1;
+    if (s >= 0 && s < a.cache.num_blocks * a.cache.block_size)
+      row = (s / a.cache.block_size) * a.cache.block_stride + (s % a.cache.block_size) * a.cache.token_stride;
+    cache_rows[tid] = row;
   }
   __syncthreads();
-  long cache_row = -1;
-  if (a.cache.keys) {
-    const int s = a.slots[t];
-    if (s >= 0 && s < a.cache.num_blocks * a.cache.block_size)
-      cache_row = (s / a.cache.block_size) * a.cache.block_stride + (s % a.cache.block_size) * a.cache.token_stride;
-  }
-  const int rotated = a.pairs / N, chunks = rotated + (a.head_dim - 2 * a.pairs) / N;
-  for (int i = tid; i < chunks * a.heads; i += kThreads) {
-    const int h = i / chunks, c = i - h * chunks;
+  const int rotated = a.pairs / N, chunks = a.chunks.d;
+  for (int i = tid; i < chunks * a.heads * tokens; i += kThreads) {
+    const int h0 = a.chunks.quotient(i), c = i - h0 * chunks;
+    const int tl = TB == 1 ? 0 : a.by_heads.quotient(h0), h = h0 - tl * a.heads, t = t0 + tl;
     head_chunk<T, N, ADJACENT>(static_cast<const T*>(a.q.data) + t * a.q.token_stride + h * a.q.head_stride,
                                static_cast<T*>(a.q_out.data) + t * a.q_out.token_stride + h * a.q_out.head_stride,
-                               nullptr, c, rotated, a.pairs, cs, sn);
+                               nullptr, c, rotated, a.pairs, cs[tl], sn[tl]);
   }
   if (a.k.data)
-    for (int i = tid; i < chunks * a.heads_kv; i += kThreads) {
-      const int h = i / chunks, c = i - h * chunks;
+    for (int i = tid; i < chunks * a.heads_kv * tokens; i += kThreads) {
+      const int h0 = a.chunks.quotient(i), c = i - h0 * chunks;
+      const int tl = TB == 1 ? 0 : a.by_heads_kv.quotient(h0), h = h0 - tl * a.heads_kv, t = t0 + tl;
+      const long row = a.cache.keys ? cache_rows[tl] : -1;
       T* out = a.k_out.data ? static_cast<T*>(a.k_out.data) + t * a.k_out.token_stride + h * a.k_out.head_stride
                             : nullptr;
-      T* kept = cache_row >= 0 ? static_cast<T*>(a.cache.keys) + cache_row + h * a.cache.head_stride : nullptr;
+      T* kept = row >= 0 ? static_cast<T*>(a.cache.keys) + row + h * a.cache.head_stride : nullptr;
       head_chunk<T, N, ADJACENT>(static_cast<const T*>(a.k.data) + t * a.k.token_stride + h * a.k.head_stride,
-                                 out, kept, c, rotated, a.pairs, cs, sn);
+                                 out, kept, c, rotated, a.pairs, cs[tl], sn[tl]);
     }
-  if (a.v.data && cache_row >= 0) {
+  if (a.v.data) {
     constexpr int V = 16 / sizeof(T);
-    const int vc = a.head_dim / V;
-    for (int i = tid; i < vc * a.heads_kv; i += kThreads) {
-      const int h = i / vc, c = i - h * vc;
-      store<T, V>(static_cast<T*>(a.cache.values) + cache_row + h * a.cache.head_stride + c * V,
-                  load<T, V>(static_cast<const T*>(a.v.data) + t * a.v.token_stride + h * a.v.head_stride + c * V));
+    const int vc = a.value_chunks.d;
+    for (int i = tid; i < vc * a.heads_kv * tokens; i += kThreads) {
+      const int h0 = a.value_chunks.quotient(i), c = i - h0 * vc;
+      const int tl = TB == 1 ? 0 : a.by_heads_kv.quotient(h0), h = h0 - tl * a.heads_kv, t = t0 + tl;
+      if (cache_rows[tl] >= 0)
+        store<T, V>(static_cast<T*>(a.cache.values) + cache_rows[tl] + h * a.cache.head_stride + c * V,
+                    load<T, V>(static_cast<const T*>(a.v.data) + t * a.v.token_stride + h * a.v.head_stride + c * V));
     }
   }
 }
 
 template <typename T, int N>
-void launch(const RotaryArgs& a, bool adjacent, hipStream_t st) {
-  if (adjacent) rotary_kernel<T, N, true><<<a.tokens, kThreads, 0, st>>>(a);
-  else rotary_kernel<T, N, false><<<a.tokens, kThreads, 0, st>>>(a);
+void launch(RotaryArgs a, bool adjacent, hipStream_t st) {
+  a.chunks.set(a.pairs / N + (a.head_dim - 2 * a.pairs) / N);
+  a.value_chunks.set(a.head_dim * sizeof(T) / 16);
+  a.by_heads.set(a.heads);
+  a.by_heads_kv.set(a.heads_kv > 0 ? a.heads_kv : 1);
+  // Four tokens to a workgroup where one would not occupy its threads, and tokens abound.  In
+  // bf16: 20000 tokens of 4/1 heads of 128 27.6 us with one, 16.0 with four; 5491 of 6/2 11.4 and
+  // 8.9; 8000 of 12/12 heads of 64 16.3 and 15.4; but 16384 of 32/8 heads of 128 82.5 and 87.7.
+  const int items = static_cast<int>(a.chunks.d * (a.heads + a.heads_kv) + a.value_chunks.d * a.heads_kv);
+  if (items <= kThreads && a.tokens >= 1024) {
+    if (adjacent) rotary_kernel<T, N, true, 4><<<ceil_div(a.tokens, 4), kThreads, 0, st>>>(a);
+    else rotary_kernel<T, N, false, 4><<<ceil_div(a.tokens, 4), kThreads, 0, st>>>(a);
+  } else {
+    if (adjacent) rotary_kernel<T, N, true, 1><<<a.tokens, kThreads, 0, st>>>(a);
+    else rotary_kernel<T, N, false, 1><<<a.tokens, kThreads, 0, st>>>(a);
+  }
 }
 
 // The widest chunk, up to 16 bytes, that divides both halves of the turned part.

@@ -16,6 +16,24 @@ using bf16_t = __bf16;
 
 constexpr int kMaxHeadDim = 256;
 
+// n / d for 0 <= n < 2^32 by a product: the round-up method for invariant divisors
+// (Granlund and Montgomery, 1994).
+struct FastDivision {
+  unsigned d, factor;
+  int shift;
+  void set(unsigned divisor) {
+    d = divisor;
+    int log = 0;
+    while ((1ull << log) < divisor) ++log;  // ceil(log2 d)
+    factor = static_cast<unsigned>((((1ull << log) - divisor) << 32) / divisor + 1);
+    shift = log;
+  }
+  __device__ __forceinline__ unsigned quotient(unsigned n) const {
+    const unsigned t = __umulhi(factor, n);
+    return shift == 0 ? n : (t + ((n - t) >> 1)) >> (shift - 1);
+  }
+};
+
 inline size_t type_size(int type) { return type == MC_TYPE_F32 ? 4 : 2; }
 
 // The 16-byte rule: every row of every head then starts where 16-byte loads may.
