@@ -524,7 +524,8 @@ enum mcDataType { MC_TYPE_F32 = 0, MC_TYPE_F16 = 1, MC_TYPE_BF16 = 2 };
 /* Rows of heads: head h of token t starts at element t * token_stride + h * head_stride
  * of `data` (device), its head_dim values are contiguous.  `data` and both strides, in
  * bytes, are multiples of 16.  One struct describes a slice of a fused projection, a
- * plain [tokens, heads, head_dim] blob or a transposed one. */
+ * plain [tokens, heads, head_dim] blob or a transposed one.  The token stride of keys and
+ * values that an attention reads (a cache's too) is 0 to 2^25 bytes. */
 typedef struct mcHeads {
   void* data;
   long token_stride;
@@ -597,7 +598,7 @@ typedef struct mcRotaryGeom {
 } mcRotaryGeom;
 
 /* frequencies [rotary_dim / 2]; positions: axis a at positions + a * axis_stride, `tokens`
- * ints each.  q -> q_out.  k (or NULL) -> k_out (or NULL) and, with a cache, the cache's
+ * ints each, axis_stride >= 0.  q -> q_out.  k (or NULL) -> k_out (or NULL) and, with a cache, the cache's
  * keys at slots[token]; v (or NULL) -> the cache's values there, unchanged.  A slot
  * outside the cache (-1: none) is not stored.  q_out == q and k_out == k are allowed
  * (same strides). */
@@ -637,8 +638,9 @@ int mcAttentionPacked(const mcAttentionGeom* geom, const mcHeads* q, const mcHea
  * more new tokens / keys (host numbers that size the launch; a request's rows beyond
  * max_q are not computed, keys beyond max_context or the table not seen).  Work over a
  * long context with few rows is cut into pieces; their partial results lie in scratch
- * that the calling thread owns (mcReleaseScratch): before the call is captured, make one
- * call of the same sizes outside. */
+ * that the calling thread owns for this stream (mcReleaseScratch): before the call is
+ * captured, make one call of the same sizes outside.  A later call there that needs more
+ * frees that scratch, so none may be made while a graph that used it is replayed. */
 int mcAttentionPaged(const mcAttentionGeom* geom, const mcHeads* q, const mcPagedCache* cache,
                      const int* block_table, int table_width, const int* q_starts,
                      const int* context_lens, int num_requests, int total_q, int max_q,

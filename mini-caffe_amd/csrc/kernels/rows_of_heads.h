@@ -62,7 +62,7 @@ inline int check_cache(const char* who, const mcPagedCache* c, int type) {
 
 // A kernel forms the offsets of the rows of a tile in 32 bits.
 inline int check_key_stride(const char* who, const char* what, long token_stride, int type) {
-  MC_REQUIRE(token_stride >= 0 && token_stride * static_cast<long>(type_size(type)) <= (1l << 25),
+  MC_REQUIRE(token_stride >= 0 && token_stride <= (1l << 25) / static_cast<long>(type_size(type)),
              "%s: %s: token_stride %ld is negative or above 2^25 bytes", who, what, token_stride);
   return 0;
 }

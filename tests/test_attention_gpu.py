@@ -576,3 +576,27 @@ def test_infinite_keys(A, kind, where):
             want = rows64(q[r:r + 1, 0], k[kept, 0], v[kept, 0], 1 / 8, [len(kept)])
             lse = torch.log(torch.exp(torch.zeros(1))) + want[1]
             check(kind, d, n, out[r:r + 1, 0], lse, want, 5.0)
+
+
+# ---- strides that a tile's 32-bit offsets could not hold ------------------------------------
+
+@pytest.mark.parametrize("kind,size", [("f32", 4), ("bf16", 2)])
+@pytest.mark.parametrize("which", ["k", "v", "cache"])
+def test_refused_key_strides(A, kind, size, which):
+    from minicaffe import MiniCaffeError
+    code = {"f32": 0, "bf16": 2}[kind]
+    dtype = torch.float32 if kind == "f32" else torch.bfloat16
+    x = torch.zeros((16, 2, 64), device="cuda", dtype=dtype)
+    c = torch.zeros((1, 16, 2, 64), device="cuda", dtype=dtype)
+    st, lens, table = ints([0, 16]), ints([16]), ints([0])
+    h = A.heads_of(x)
+    geom = A.AttentionGeom(code, 2, 2, 64, 1, 0.125)
+    for stride in (-128, 2 ** 25 // size + 16 // size, 2 ** 62):
+        with pytest.raises(MiniCaffeError, match="token_stride"):
+            if which == "cache":
+                bad = A.PagedCache(c.data_ptr(), c.data_ptr(), 1, 16, c.stride(0), stride, c.stride(2))
+                A.attention_paged(geom, h, bad, table.data_ptr(), 1, st.data_ptr(), lens.data_ptr(), 1, 16, 16, 16, h)
+            else:
+                bad = A.Heads(x.data_ptr(), stride, 64)
+                A.attention_packed(geom, h, bad if which == "k" else h, bad if which == "v" else h, st.data_ptr(), st.data_ptr(),
+                                   1, 16, 16, h)

@@ -175,3 +175,12 @@ def test_refusals(A):
     call(tokens=0)
     with pytest.raises(ValueError):
         call(sections=())
+
+
+def test_refused_axis_stride(A):
+    from minicaffe import MiniCaffeError
+    x, f = torch.zeros((4, 2, 64), device="cuda"), torch.zeros(32, device="cuda")
+    pos = torch.zeros((2, 4), dtype=torch.int32, device="cuda")
+    h = A.heads_of(x)
+    with pytest.raises(MiniCaffeError, match="axis_stride"):
+        A.rotary(A.rotary_geom(0, 2, 0, 64, 64, [16, 16]), f.data_ptr(), pos.data_ptr(), -4, 4, h, h)
