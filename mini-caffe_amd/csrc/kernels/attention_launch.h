@@ -72,9 +72,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttentionArgs
         l == 0.f ? -INFINITY : (top - kLift<T> + log2f(l)) * 0.69314718f;
 }
 
-template <typename T, int DP, bool PAGED, int W>
+template <typename T, int DP, bool PAGED, int W, bool LEAN = false>
 int launch_tiles(AttentionArgs a, hipStream_t st) {
-  using S = TileShape<T, DP, W>;
+  using S = TileShape<T, DP, W, LEAN>;
   const long group = a.group.d;
   a.tile_rows = S::kRows;
   a.tiles = static_cast<int>(a.total_q * group / S::kRows) + a.num;
@@ -90,7 +90,7 @@ int launch_tiles(AttentionArgs a, hipStream_t st) {
     // the GPU knows; about half a tile per sequence is not full.
     const long tiles = a.num == 1 ? ceil_div(a.total_q * group, S::kRows)
                                   : std::max<long>(a.total_q * group / S::kRows + (a.num + 1) / 2, std::min(a.num, a.total_q));
-    const long items = tiles * a.heads_kv, slots = (W == 8 || DP > 128 ? 1 : 2) * kNumCu;
+    const long items = tiles * a.heads_kv, slots = S::kPerCu * kNumCu;
     const long sums = static_cast<long>(a.total_q) * a.heads * DP * 8;  // bytes of one piece, both ways
     const int most = std::max(1, std::min(a.max_context / (4 * S::kKeys), kMostPieces));
     int wanted = 1;
@@ -113,10 +113,10 @@ int launch_tiles(AttentionArgs a, hipStream_t st) {
   MC_REQUIRE(blocks <= INT_MAX, "attention: %ld workgroups", blocks);
   const unsigned grid = static_cast<unsigned>(blocks);
   if constexpr (!PAGED) {
-    attention_tile_kernel<T, DP, Source::kPacked, W><<<grid, 64 * W, 0, st>>>(a);
+    attention_tile_kernel<T, DP, Source::kPacked, W, LEAN><<<grid, 64 * W, 0, st>>>(a);
   } else {
-    if (a.block.d % S::kRun == 0) attention_tile_kernel<T, DP, Source::kRuns, W><<<grid, 64 * W, 0, st>>>(a);
-    else attention_tile_kernel<T, DP, Source::kPaged, W><<<grid, 64 * W, 0, st>>>(a);
+    if (a.block.d % S::kRun == 0) attention_tile_kernel<T, DP, Source::kRuns, W, LEAN><<<grid, 64 * W, 0, st>>>(a);
+    else attention_tile_kernel<T, DP, Source::kPaged, W, LEAN><<<grid, 64 * W, 0, st>>>(a);
   }
   MC_LAUNCH_CHECK();
   if (PAGED && a.pieces > 1) {
@@ -185,6 +185,19 @@ int launch_rows(const AttentionArgs& a, hipStream_t st) {
     if (rows / a.num >= 512 && keys >= 512 &&
         (PAGED || rows * a.heads_kv >= 1l * kNumCu * TileShape<T, DP, 8>::kRows))
       return launch_tiles<T, DP, PAGED, 8>(a, st);
+  // Three workgroups a CU, with smaller tiles, where there are workgroups for it: many short
+  // sequences then hide each other's beginnings and ends.  Lean and not, us, heads of 64/96/128 in
+  // bf16: 24 prompts of 100 to 1500, 32/8 heads, 5032 workgroups, 136/192/234 and 153/203/238; 40 of 50
+  // to 300, 2056 workgroups, 28/37/45 and 33/43/49; but 4 of 1024, 1056, 43/52/61 and 39/52/59; a
+  // prompt of 2048, 520, 43/55/69 and 39/51/56.  And where they fit at once, all of a length, and two
+  // a CU would take turns: 9 images of 577 cells, 16 heads, 720 workgroups, 28/40/45 and 34/46/51.
+  // fp32 of 64: the 40 sequences 76 and 79; 5 images of 1369, 12 heads, 660 workgroups, 170 and 200.
+  // (Through a block table the addresses take more registers: heads of 128 would spill 31.)
+  if constexpr (!PAGED && (sizeof(T) == 2 ? DP <= 128 : DP == 64)) {
+    const long most = (rows / TileShape<T, DP>::kRows + a.num) * a.heads_kv;
+    if (most >= 8l * kNumCu || (!a.causal && most > 2 * kNumCu && most <= 3 * kNumCu))
+      return launch_tiles<T, DP, PAGED, 4, true>(a, st);
+  }
   return launch_tiles<T, DP, PAGED, 4>(a, st);
 }
 

@@ -45,11 +45,13 @@ struct Product {
   }
 };
 
-template <typename T, int DP, int W = 4>  // W: wavefronts of the workgroup
+// W: wavefronts of the workgroup.  LEAN: tiles of 32 keys (fp32: one tile in LDS), so that a SIMD has
+// registers for three wavefronts and a CU room for three workgroups.
+template <typename T, int DP, int W = 4, bool LEAN = false>
 struct TileShape {
   static constexpr int kRows = 32 * W;
   static constexpr int kRowBytes = DP * static_cast<int>(sizeof(T));
-  static constexpr int kKeys = sizeof(T) == 2 && kRowBytes <= 256 ? 64 : 32;  // keys of a tile
+  static constexpr int kKeys = sizeof(T) == 2 && kRowBytes <= 256 && !LEAN ? 64 : 32;  // keys of a tile
   static constexpr int kChunks = kRowBytes / 16;               // 16-byte chunks of a row
   // LDS rows: an odd number of chunks apart for K, so that 16 lanes that read one chunk of
   // 16 rows meet all banks; V's rows so that the 4 (16 bits) or 2 (32 bits, four rows
@@ -71,10 +73,15 @@ struct TileShape {
   static constexpr int kOutStride = kRowBytes + 16;
   // Two tiles in LDS, one read while the other is written; one where two would leave a CU to a
   // single workgroup of four wavefronts (terms of 96 and 128 values).
-  static constexpr int kBuffers = kSplit && DP > 64 && W < 8 ? 1 : 2;
+  static constexpr int kBuffers = kSplit && (DP > 64 || LEAN) && W < 8 ? 1 : 2;
   static constexpr int kTiles = kBuffers * (kKTile + kVTile);
   static constexpr int kLds = kTiles > 32 * W * kOutStride ? kTiles : 32 * W * kOutStride;
   static_assert(kKeys % kPass == 0, "a pass over the workgroup loads more than a tile");
+  // Wavefronts of a SIMD that the registers are shared out for.  16-bit rows of 192 values: two
+  // take all 256 of them, and twelve heads of five times 1369 rows in bf16 150 us; one 211.  (Of 256
+  // values two would have to spill: 265, one 241.)
+  static constexpr int kPerSimd = LEAN ? 3 : DP <= 128 || (DP <= 192 && sizeof(T) == 2) ? 2 : 1;
+  static constexpr int kPerCu = W == 8 ? 1 : kPerSimd;  // workgroups
 };
 
 // Where the keys are.
@@ -153,10 +160,9 @@ __device__ __forceinline__ void scores_by_terms(const char* lds_k, const uintx4 
 }
 
 // Scores of the tile's keys against the wavefront's rows, in blocks of 32 keys.
-template <typename T, int DP>
+template <typename T, int DP, int SUB>
 __device__ __forceinline__ void scores(const char* lds_k, const floatx4* q, floatx16* c, int lane) {
   using S = TileShape<T, DP>;
-  constexpr int SUB = S::kKeys / 32;
   const char* at = lds_k + (lane & 31) * S::kKStride + (lane >> 5) * 16;
 #pragma unroll
   for (int u = 0; u < SUB; ++u) c[u] = floatx16{};
@@ -195,10 +201,9 @@ __device__ __forceinline__ bool finite16(short x, unsigned short exponent) {
 
 // O^T += V^T P^T for the tile's keys, p: the lane's weights.
 // SAFE: infinities and NaN of V count as 0 here.
-template <typename T, int DP, bool SAFE>
+template <typename T, int DP, int SUB, bool SAFE>
 __device__ __forceinline__ void weighted_sum(const char* lds_v, const floatx16* p, floatx16* o, int lane) {
   using S = TileShape<T, DP>;
-  constexpr int SUB = S::kKeys / 32;
   if constexpr (sizeof(T) == 2) {
     constexpr unsigned short kExponent = __is_same(T, bf16_t) ? 0x7f80 : 0x7c00;
     const char* at = lds_v + (4 * (lane >> 5) + ((lane & 15) >> 2)) * S::kVStride +
@@ -395,10 +400,10 @@ __device__ __forceinline__ void store_out(const AttentionArgs& a, const floatx16
     }
 }
 
-template <typename T, int DP, Source SRC, int W>
-__global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attention_tile_kernel(
+template <typename T, int DP, Source SRC, int W, bool LEAN>
+__global__ __launch_bounds__(64 * W, (TileShape<T, DP, W, LEAN>::kPerSimd)) void attention_tile_kernel(
     const AttentionArgs a) {
-  using S = TileShape<T, DP, W>;
+  using S = TileShape<T, DP, W, LEAN>;
   constexpr bool PAGED = SRC != Source::kPacked;
   constexpr int KT = S::kKeys, SUB = KT / 32;
   __shared__ __attribute__((aligned(16))) char lds[S::kLds];
@@ -622,8 +627,8 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attention_tile_kern
       const char* const now_v = lds_v + buffer * S::kVTile;
       floatx16 s[SUB];
       if (work) {
-        if constexpr (!S::kSplit) scores<T, DP>(now_k, q, s, lane);
-        else if constexpr (SAFE) scores<T, DP>(now_k, q_safe, s, lane);
+        if constexpr (!S::kSplit) scores<T, DP, SUB>(now_k, q, s, lane);
+        else if constexpr (SAFE) scores<T, DP, SUB>(now_k, q_safe, s, lane);
         else scores_by_terms<DP>(now_k, q_terms, s, lane);
       }
       if (S::kBuffers == 2 && at + KT < end) {
@@ -646,7 +651,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attention_tile_kern
         }
         softmax_step<T, DP, SUB>(s, o, run, a.scale_log2);
         if constexpr (S::kSplit && !SAFE) weighted_sum_by_terms<DP>(now_v, s[0], o, lane);
-        else weighted_sum<T, DP, SAFE>(now_v, s, o, lane);
+        else weighted_sum<T, DP, SUB, SAFE>(now_v, s, o, lane);
         if (SAFE) add_not_finite<T, DP>(now_v, min(min(limit, end) - at, KT), valid, o, lane);
       }
       __syncthreads();

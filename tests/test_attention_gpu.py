@@ -600,3 +600,54 @@ def test_refused_key_strides(A, kind, size, which):
                 bad = A.Heads(x.data_ptr(), stride, 64)
                 A.attention_packed(geom, h, bad if which == "k" else h, bad if which == "v" else h, st.data_ptr(), st.data_ptr(),
                                    1, 16, 16, h)
+
+
+# ---- enough workgroups for three to a CU, and rows of 192 values ------------------------------
+
+def check_heads(q, k, v, lengths, causal, out, lse, heads):
+    """As check_packed, as many key heads as query heads, `heads` of them."""
+    check_packed(q[:, heads], k[:, heads], v[:, heads], lengths, lengths, causal, out[:, heads], lse[heads])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_many_workgroups(A, kind, dim, causal):
+    """Short sequences with many key heads: 2048 workgroups and more; an empty sequence, one token, and ragged ends."""
+    g = torch.Generator(device="cuda").manual_seed(31)
+    lengths = [(11 * i) % 43 for i in range(66)] + [131, 65, 64, 33, 1]
+    n = sum(lengths)
+    q, k, v = (randn(g, n, 32, dim, kind=kind) for _ in range(3))
+    out, lse = packed(A, q, k, v, lengths, lengths, causal)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    check_heads(q, k, v, lengths, causal, out, lse, [0, 13, 31])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+def test_packed_workgroups_at_once(A, kind, dim):
+    """Between 512 and 768 workgroups of equal length, not causal; an infinity and a NaN in two sequences' values."""
+    g = torch.Generator(device="cuda").manual_seed(32)
+    lengths = [200] * 12
+    q, k, v = (randn(g, 2400, 20, dim, kind=kind) for _ in range(3))
+    clean, clean_lse = packed(A, q, k, v, lengths, lengths, False)
+    check_heads(q, k, v, lengths, False, clean, clean_lse, [0, 3, 19])
+    poisoned = v.clone()
+    poisoned[250, 3, 5] = float("inf")
+    poisoned[1999, 0, 0] = float("nan")
+    out, lse = packed(A, q, k, poisoned, lengths, lengths, False)
+    assert torch.isposinf(out[200:400, 3, 5]).all() and torch.isnan(out[1800:2000, 0, 0]).all()
+    out[200:400, 3, 5] = clean[200:400, 3, 5]
+    out[1800:2000, 0, 0] = clean[1800:2000, 0, 0]
+    check_heads(q, k, v, lengths, False, out, lse, [0, 3, 19])
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [136, 192])
+@pytest.mark.parametrize("lengths", [[1], [33, 0, 128, 257], [700]])
+def test_packed_192(A, kind, dim, lengths):
+    g = torch.Generator(device="cuda").manual_seed(33)
+    n = sum(lengths)
+    q, k, v = (randn(g, n, h, dim, kind=kind) for h in (4, 2, 2))
+    out, lse = packed(A, q, k, v, lengths, lengths, True)
+    check_packed(q, k, v, lengths, lengths, True, out, lse)
