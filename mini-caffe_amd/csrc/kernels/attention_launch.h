@@ -161,7 +161,10 @@ int launch_few_rows(AttentionArgs a, hipStream_t st) {
 // into LDS.  In bf16, 32/8 heads of 128: 8192 causal tokens 566 us with four, 531 with eight; a
 // chunk of 512 over 32768 334 and 309; sequences of 1024, not causal, 417 and 408; of 512, 250
 // and 253; of 128, 121 and 147 (a tile's unused rows, and a workgroup alone on its CU has
-// nothing to do while it begins and ends).
+// nothing to do while it begins and ends).  Wider rows, whose copies are wider, gain sooner: heads
+// of 192/256, 4096 causal tokens, 32/8, 244/310 and 206/270; eight images of 512, 16 heads,
+// 45/59 and 39/53; but 40 sequences of 50 to 300, 16 heads, 63/86 and 70/94, one of 300, 16/4, 18/24 and
+// 19/26.
 template <typename T, int DP, bool PAGED>
 int launch_rows(const AttentionArgs& a, hipStream_t st) {
   const long group = a.group.d;
@@ -172,10 +175,12 @@ int launch_rows(const AttentionArgs& a, hipStream_t st) {
       if (most <= 32) return launch_few_rows<T, DP, 2>(a, st);
   }
   const long rows = a.total_q * group, keys = PAGED ? a.max_context : a.total_k / a.num;
-  if constexpr (sizeof(T) == 2 && DP <= 128) {  // (wider rows leave one wavefront to a SIMD)
-    if (rows / a.num >= 1024 && keys >= 1024 &&
-        (PAGED || rows * a.heads_kv >= 2l * kNumCu * TileShape<T, DP, 8>::kRows))
-      return launch_tiles<T, DP, PAGED, 8>(a, st);
+  if constexpr (sizeof(T) == 2) {
+    constexpr bool kWide = DP > 128;
+    const long enough = kWide && !PAGED ? 512 : 1024, tiles = kWide ? 1 : 4;
+    if (rows / a.num >= enough && keys >= enough / (kWide && !PAGED ? a.group.d : 1) &&
+        (PAGED || rows * a.heads_kv >= tiles * kNumCu * TileShape<T, DP>::kRows))
+      return launch_tiles<T, DP, PAGED, 8, (DP > 192)>(a, st);
   }
   // fp32 by terms of more than 64 values has one tile in LDS with four wavefronts and two with
   // eight: 4096 causal tokens, 32/8 heads of 128 721 us and 625; five images of 273 to 1369 cells,
@@ -198,6 +203,12 @@ int launch_rows(const AttentionArgs& a, hipStream_t st) {
     if (most >= 8l * kNumCu || (!a.causal && most > 2 * kNumCu && most <= 3 * kNumCu))
       return launch_tiles<T, DP, PAGED, 4, true>(a, st);
   }
+  // Rows of 256 values: K and V in turn only where a CU gets two workgroups.  512 workgroups of 40
+  // sequences of 50 to 300, 16 heads, 86 us and 116; but eight chunks of 64 over 1000, 16/4 heads, 80
+  // workgroups, 48 and 41.
+  if constexpr (sizeof(T) == 2 && DP > 192)
+    if ((rows / TileShape<T, DP>::kRows + a.num) * a.heads_kv > kNumCu)
+      return launch_tiles<T, DP, PAGED, 4, true>(a, st);
   return launch_tiles<T, DP, PAGED, 4>(a, st);
 }
 

@@ -45,8 +45,9 @@ struct Product {
   }
 };
 
-// W: wavefronts of the workgroup.  LEAN: tiles of 32 keys (fp32: one tile in LDS), so that a SIMD has
-// registers for three wavefronts and a CU room for three workgroups.
+// W: wavefronts of the workgroup.  LEAN: one more of the workgroups of four fits a CU: by tiles of 32
+// keys (fp32: one tile in LDS) for rows of at most 128 values, three; in 16 bits by K and V carried
+// in the same registers, one after the other, for rows of 256, two.
 template <typename T, int DP, int W = 4, bool LEAN = false>
 struct TileShape {
   static constexpr int kRows = 32 * W;
@@ -77,10 +78,11 @@ struct TileShape {
   static constexpr int kTiles = kBuffers * (kKTile + kVTile);
   static constexpr int kLds = kTiles > 32 * W * kOutStride ? kTiles : 32 * W * kOutStride;
   static_assert(kKeys % kPass == 0, "a pass over the workgroup loads more than a tile");
-  // Wavefronts of a SIMD that the registers are shared out for.  16-bit rows of 192 values: two
-  // take all 256 of them, and twelve heads of five times 1369 rows in bf16 150 us; one 211.  (Of 256
-  // values two would have to spill: 265, one 241.)
-  static constexpr int kPerSimd = LEAN ? 3 : DP <= 128 || (DP <= 192 && sizeof(T) == 2) ? 2 : 1;
+  static constexpr bool kInTurn = LEAN && sizeof(T) == 2 && DP > 192;
+  // Wavefronts of a SIMD that the registers are shared out for.  16-bit rows of 192 values: two take
+  // all of them, and twelve heads of five times 1369 rows in bf16 148 us; one 211.  Of 256 values
+  // one 241, two 265 (what does not fit is spilled), two in turn 195.
+  static constexpr int kPerSimd = DP <= 128 ? (LEAN ? 3 : 2) : sizeof(T) == 2 && (DP <= 192 || LEAN) ? 2 : 1;
   static constexpr int kPerCu = W == 8 ? 1 : kPerSimd;  // workgroups
 };
 
@@ -481,7 +483,8 @@ __global__ __launch_bounds__(64 * W, (TileShape<T, DP, W, LEAN>::kPerSimd)) void
   const int run_row = lane / S::kLanes;  // of the rows that the wavefront loads
   const unsigned k_off = (SRC == Source::kRuns ? run_row : pass_row) * static_cast<unsigned>(k_stride) + chunk_at;
   const unsigned v_off = (SRC == Source::kRuns ? run_row : pass_row) * static_cast<unsigned>(v_stride) + chunk_at;
-  floatx4 stage_k[S::kStage], stage_v[S::kStage];
+  floatx4 stage_k[S::kStage], stage_other[S::kInTurn ? 1 : S::kStage];
+  floatx4* const stage_v = S::kInTurn ? stage_k : stage_other;
   constexpr unsigned long kAllValid = KT == 64 ? ~0ul : (1ul << KT) - 1;
   // kRuns: 64 entries of the block table, one per lane, from block `window` on, and those 32
   // further on, asked for long before they are used.  A tile spans 32 blocks at most.
@@ -498,23 +501,27 @@ __global__ __launch_bounds__(64 * W, (TileShape<T, DP, W, LEAN>::kPerSimd)) void
   auto exist = [&](int tile_begin) {  // bit k: the tile's key k has a block
     return __ballot(cache_row(a, table, min(tile_begin + lane % KT, end - 1)) >= 0) & kAllValid;
   };
-  auto fetch = [&](int tile_begin) {  // keys past the end repeat the last one
+  // what is carried: 1 K, 2 V, 3 both
+  const std::integral_constant<int, S::kInTurn ? 1 : 3> keys_first;
+  const std::integral_constant<int, 2> values_next;
+  auto fetch = [&](int tile_begin, auto which) {  // keys past the end repeat the last one
+    constexpr bool K = decltype(which)::value & 1, V = decltype(which)::value & 2;
     if constexpr (SRC == Source::kPacked) {
       const char* kt = kbase + tile_begin * k_stride;
       const char* vt = vbase + tile_begin * v_stride;
       if (tile_begin + KT <= end) {
 #pragma unroll
         for (int i = 0; i < S::kStage; ++i) {
-          stage_k[i] = *reinterpret_cast<const floatx4*>(kt + i * S::kPass * k_stride + k_off);
-          stage_v[i] = *reinterpret_cast<const floatx4*>(vt + i * S::kPass * v_stride + v_off);
+          if constexpr (K) stage_k[i] = *reinterpret_cast<const floatx4*>(kt + i * S::kPass * k_stride + k_off);
+          if constexpr (V) stage_v[i] = *reinterpret_cast<const floatx4*>(vt + i * S::kPass * v_stride + v_off);
         }
       } else {
         const int last = end - 1 - tile_begin;
 #pragma unroll
         for (int i = 0; i < S::kStage; ++i) {
           const unsigned r = min(pass_row + i * S::kPass, last);
-          stage_k[i] = *reinterpret_cast<const floatx4*>(kt + (r * static_cast<unsigned>(k_stride) + chunk_at));
-          stage_v[i] = *reinterpret_cast<const floatx4*>(vt + (r * static_cast<unsigned>(v_stride) + chunk_at));
+          if constexpr (K) stage_k[i] = *reinterpret_cast<const floatx4*>(kt + (r * static_cast<unsigned>(k_stride) + chunk_at));
+          if constexpr (V) stage_v[i] = *reinterpret_cast<const floatx4*>(vt + (r * static_cast<unsigned>(v_stride) + chunk_at));
         }
       }
     } else if constexpr (SRC == Source::kRuns) {
@@ -534,22 +541,23 @@ __global__ __launch_bounds__(64 * W, (TileShape<T, DP, W, LEAN>::kPerSimd)) void
         unsigned off = k_off;
         if (tile_begin + KT > end)
           off = min(run_row, end - 1 - static_cast<int>(key)) * static_cast<unsigned>(k_stride) + chunk_at;
-        stage_k[i] = *reinterpret_cast<const floatx4*>(kbase + at + off);
-        stage_v[i] = *reinterpret_cast<const floatx4*>(vbase + at + off);
+        if constexpr (K) stage_k[i] = *reinterpret_cast<const floatx4*>(kbase + at + off);
+        if constexpr (V) stage_v[i] = *reinterpret_cast<const floatx4*>(vbase + at + off);
       }
     } else {
       const long at = max(cache_row(a, table, min(tile_begin + lane % KT, end - 1)), 0l) * static_cast<long>(sizeof(T));
 #pragma unroll
       for (int i = 0; i < S::kStage; ++i) {
         const long from = __shfl(at, pass_row + i * S::kPass, 64) + chunk_at;
-        stage_k[i] = *reinterpret_cast<const floatx4*>(kbase + from);
-        stage_v[i] = *reinterpret_cast<const floatx4*>(vbase + from);
+        if constexpr (K) stage_k[i] = *reinterpret_cast<const floatx4*>(kbase + from);
+        if constexpr (V) stage_v[i] = *reinterpret_cast<const floatx4*>(vbase + from);
       }
     }
   };
   bool strange = false;  // by terms: some value was not finite, and went in as zero
-  auto write = [&](auto safe, int buffer) {
+  auto write = [&](auto safe, auto which, int buffer) {
     constexpr bool TERMS = S::kSplit && !decltype(safe)::value;
+    constexpr bool K = decltype(which)::value & 1, V = decltype(which)::value & 2;
     char* const to_k = lds_k + buffer * S::kKTile;
     char* const to_v = lds_v + buffer * S::kVTile;
     if constexpr (TERMS) {
@@ -574,13 +582,13 @@ __global__ __launch_bounds__(64 * W, (TileShape<T, DP, W, LEAN>::kPerSimd)) void
     } else {
 #pragma unroll
       for (int i = 0; i < S::kStage; ++i) {
-        *reinterpret_cast<floatx4*>(to_k + (pass_row + i * S::kPass) * S::kKStride + chunk * 16) = stage_k[i];
-        *reinterpret_cast<floatx4*>(to_v + (pass_row + i * S::kPass) * S::kVStride + chunk * 16) = stage_v[i];
+        if constexpr (K) *reinterpret_cast<floatx4*>(to_k + (pass_row + i * S::kPass) * S::kKStride + chunk * 16) = stage_k[i];
+        if constexpr (V) *reinterpret_cast<floatx4*>(to_v + (pass_row + i * S::kPass) * S::kVStride + chunk * 16) = stage_v[i];
       }
     }
   };
-  auto put = [&](auto safe, int buffer) {
-    if (there) write(safe, buffer);
+  auto put = [&](auto safe, auto which, int buffer) {
+    if (there) write(safe, which, buffer);
   };
   open_window(begin);
   // Blocks that do not exist are looked for once; where there is one, the safe pass leaves them out.
@@ -590,7 +598,7 @@ __global__ __launch_bounds__(64 * W, (TileShape<T, DP, W, LEAN>::kPerSimd)) void
     for (int b = a.block.quotient(begin) + tid; b <= last; b += 64 * W)
       missing |= static_cast<unsigned>(table[b]) >= static_cast<unsigned>(a.cache.num_blocks);
   }
-  if (begin < end) fetch(begin);  // (asked for before the wavefronts wait for each other)
+  if (begin < end) fetch(begin, keys_first);  // (asked for before the wavefronts wait for each other)
   if (PAGED && begin < end) missing = __syncthreads_or(missing);
 
   floatx16 o[DP / 32];
@@ -606,7 +614,7 @@ __global__ __launch_bounds__(64 * W, (TileShape<T, DP, W, LEAN>::kPerSimd)) void
     if (begin >= end) return;
     if (SAFE) {
       open_window(begin);
-      fetch(begin);
+      fetch(begin, keys_first);
     }
     if constexpr (SAFE && S::kSplit) {
 #pragma unroll
@@ -615,10 +623,14 @@ __global__ __launch_bounds__(64 * W, (TileShape<T, DP, W, LEAN>::kPerSimd)) void
     if (!there && chunk < S::kChunks) {  // chunks past head_dim: zero once
 #pragma unroll
       for (int i = 0; i < S::kStage; ++i) stage_k[i] = stage_v[i] = floatx4{};
-      for (int b = 0; b < S::kBuffers; ++b) write(safe, b);
+      for (int b = 0; b < S::kBuffers; ++b) write(safe, std::integral_constant<int, 3>(), b);
     }
-    put(safe, 0);
-    if (begin + KT < end) fetch(begin + KT);
+    put(safe, keys_first, 0);
+    if constexpr (S::kInTurn) {
+      fetch(begin, values_next);
+      put(safe, values_next, 0);
+    }
+    if (begin + KT < end) fetch(begin + KT, keys_first);
     __syncthreads();
     int buffer = 0;
     for (int at = begin; at < end; at += KT) {
@@ -632,8 +644,9 @@ __global__ __launch_bounds__(64 * W, (TileShape<T, DP, W, LEAN>::kPerSimd)) void
         else scores_by_terms<DP>(now_k, q_terms, s, lane);
       }
       if (S::kBuffers == 2 && at + KT < end) {
-        put(safe, buffer ^ 1);
-        if (at + 2 * KT < end) fetch(at + 2 * KT);
+        put(safe, keys_first, buffer ^ 1);
+        if constexpr (S::kInTurn) fetch(at + KT, values_next);
+        else if (at + 2 * KT < end) fetch(at + 2 * KT, keys_first);
       }
       if (work) {
         const bool masked = at + KT > low || (SAFE && PAGED && missing);
@@ -654,12 +667,18 @@ __global__ __launch_bounds__(64 * W, (TileShape<T, DP, W, LEAN>::kPerSimd)) void
         else weighted_sum<T, DP, SUB, SAFE>(now_v, s, o, lane);
         if (SAFE) add_not_finite<T, DP>(now_v, min(min(limit, end) - at, KT), valid, o, lane);
       }
+      if constexpr (S::kInTurn) {
+        if (at + KT < end) {
+          put(safe, values_next, buffer ^ 1);
+          if (at + 2 * KT < end) fetch(at + 2 * KT, keys_first);
+        }
+      }
       __syncthreads();
       if constexpr (S::kBuffers == 2) {
         buffer ^= 1;
       } else if (at + KT < end) {
-        put(safe, 0);
-        if (at + 2 * KT < end) fetch(at + 2 * KT);
+        put(safe, keys_first, 0);
+        if (at + 2 * KT < end) fetch(at + 2 * KT, keys_first);
         __syncthreads();
       }
     }

@@ -651,3 +651,38 @@ def test_packed_192(A, kind, dim, lengths):
     q, k, v = (randn(g, n, h, dim, kind=kind) for h in (4, 2, 2))
     out, lse = packed(A, q, k, v, lengths, lengths, True)
     check_packed(q, k, v, lengths, lengths, True, out, lse)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [136, 192, 200, 256])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_wide_rows_and_many(A, kind, dim, causal):
+    """Rows of more than 128 values and enough of them for eight wavefronts: 512 queries a sequence, 512 workgroups of 128;
+    an infinity in one sequence's values."""
+    g = torch.Generator(device="cuda").manual_seed(34)
+    lengths = [530, 700, 0, 812, 601]
+    n = sum(lengths)
+    q, k, v = (randn(g, n, 24, dim, kind=kind) for _ in range(3))
+    out, lse = packed(A, q, k, v, lengths, lengths, causal)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    check_heads(q, k, v, lengths, causal, out, lse, [0, 23])
+    poisoned = v.clone()
+    poisoned[530, 7, dim - 1] = float("inf")             # the second sequence's first key: all of its rows see it
+    again, _ = packed(A, q, k, poisoned, lengths, lengths, causal)
+    rows = slice(530, 530 + 700)
+    assert torch.isposinf(again[rows, 7, dim - 1]).all()
+    again[rows, 7, dim - 1] = out[rows, 7, dim - 1]
+    check_heads(q, k, v, lengths, causal, again, lse, [7])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [192, 256])
+@pytest.mark.parametrize("block", [16, 24, 7])
+def test_paged_wide_chunks(A, kind, dim, block):
+    """Chunks over a paged cache, rows of more than 128 values: four wavefronts, and eight where there are 1024 rows."""
+    g = torch.Generator(device="cuda").manual_seed(35)
+    for q_lens, contexts in (([40, 0, 3, 129], [300, 50, 3, 700]), ([300], [1500])):
+        keys, values, table, ks, vs = make_cache(g, contexts, block, 1, dim, kind)
+        q = randn(g, sum(q_lens), 4, dim, kind=kind)
+        out, lse = paged(A, q, keys, values, table, q_lens, contexts)
+        check_paged(q, ks, vs, q_lens, contexts, out, lse)
