@@ -192,15 +192,16 @@ int launch_rows(const AttentionArgs& a, hipStream_t st) {
       return launch_tiles<T, DP, PAGED, 8>(a, st);
   // Three workgroups a CU, with smaller tiles, where there are workgroups for it: many short
   // sequences then hide each other's beginnings and ends.  Lean and not, us, heads of 64/96/128 in
-  // bf16: 24 prompts of 100 to 1500, 32/8 heads, 5032 workgroups, 136/192/234 and 153/203/238; 40 of 50
-  // to 300, 2056 workgroups, 28/37/45 and 33/43/49; but 4 of 1024, 1056, 43/52/61 and 39/52/59; a
-  // prompt of 2048, 520, 43/55/69 and 39/51/56.  And where they fit at once, all of a length, and two
-  // a CU would take turns: 9 images of 577 cells, 16 heads, 720 workgroups, 28/40/45 and 34/46/51.
-  // fp32 of 64: the 40 sequences 76 and 79; 5 images of 1369, 12 heads, 660 workgroups, 170 and 200.
-  // (Through a block table the addresses take more registers: heads of 128 would spill 31.)
-  if constexpr (!PAGED && (sizeof(T) == 2 ? DP <= 128 : DP == 64)) {
+  // bf16: 24 prompts of 100 to 1500, 32/8 heads, 5032 workgroups, 136/192/234 and 153/203/238; 80
+  // chunks of 50 to 300 over as many, 16 heads, 3120 workgroups, 40/50/55 and 49/60/64; 40 of them,
+  // not causal, packed, 1584, 24/34/40 and 28/38/42; a prompt of 4096, 1032, 97/134/165 and
+  // 107/142/163; 8 of 1024, not causal, 16 heads, 1152, 54/79/95 and 59/79/90; but a prompt of 2048, 520,
+  // 43/55/69 and 39/51/56.  And where they fit at once, all of a length, and two a CU would take
+  // turns: 9 images of 577 cells, 16 heads, 720 workgroups, 28/40/45 and 34/46/51.
+  // fp32 of 64: the 80 chunks 95 and 104; 5 images of 1369, 12 heads, 660 workgroups, 170 and 200.
+  if constexpr (sizeof(T) == 2 ? DP <= 128 : DP == 64) {
     const long most = (rows / TileShape<T, DP>::kRows + a.num) * a.heads_kv;
-    if (most >= 8l * kNumCu || (!a.causal && most > 2 * kNumCu && most <= 3 * kNumCu))
+    if (most >= (DP <= 96 ? 4 : 5) * kNumCu || (!a.causal && most > 2 * kNumCu && most <= 3 * kNumCu))
       return launch_tiles<T, DP, PAGED, 4, true>(a, st);
   }
   // Rows of 256 values: K and V in turn only where a CU gets two workgroups.  512 workgroups of 40

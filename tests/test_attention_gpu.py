@@ -686,3 +686,30 @@ def test_paged_wide_chunks(A, kind, dim, block):
         q = randn(g, sum(q_lens), 4, dim, kind=kind)
         out, lse = paged(A, q, keys, values, table, q_lens, contexts)
         check_paged(q, ks, vs, q_lens, contexts, out, lse)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("block", [16, 5])
+def test_paged_many_chunks(A, kind, dim, block):
+    """Chunks of many requests, 1280 workgroups and more; a block that does not exist in one of them."""
+    g = torch.Generator(device="cuda").manual_seed(36)
+    q_lens = [(13 * i) % 47 for i in range(47)]
+    contexts = [n + (29 * i) % 90 for i, n in enumerate(q_lens)]
+    keys, values, table, ks, vs = make_cache(g, contexts, block, 28, dim, kind, fill=0.0)
+    q = randn(g, sum(q_lens), 28, dim, kind=kind)
+    out, lse = paged(A, q, keys, values, table, q_lens, contexts)
+    some = [0, 27]
+    check_paged(q[:, some], [k[:, some] for k in ks], [v[:, some] for v in vs], q_lens, contexts, out[:, some], lse[some])
+    at = 40                                              # its first block: those keys are left out
+    assert contexts[at] > 2 * block and q_lens[at] > 0
+    table[at, 0] = -1
+    again, again_lse = paged(A, q, keys, values, table, q_lens, contexts)
+    starts = starts_of(q_lens)
+    mine = slice(starts[at], starts[at + 1])
+    rest = [n - block for n in contexts[at:at + 1]]
+    check_paged(q[mine][:, some], [ks[at][block:, some]], [vs[at][block:, some]], [q_lens[at]], rest, again[mine][:, some],
+                again_lse[some, mine])
+    keep = torch.ones(len(q), dtype=torch.bool, device="cuda")
+    keep[mine] = False
+    assert torch.equal(again[keep], out[keep]) and torch.equal(again_lse[:, keep], lse[:, keep])
