@@ -134,7 +134,7 @@ int launch_few_rows(AttentionArgs a, hipStream_t st) {
   // wide), so that long and short contexts even out.  In bf16, with 3/4/6/8 times as many
   // workgroups as CUs: 64 x 8192, 32/8 heads of 128 250/237/237/238 us; 10 x 20000, 16/2 of 64
   // 23/22/24/31; 9 x 3089, 24/12 of 256 51/59/63/63.  But of two tiles per wavefront at least, or
-  // one where all are at work at once (1 x 513, 16/4 of 128 9.1 us, two tiles 9.9; 16 x 1000, 32/8
+  // one where all are at work at once (1 x 513, 16/4 of 80 in fp16 9.1 us, two tiles 9.9; 16 x 1000, 32/8
   // 19.4 and 16.0), and with few requests no more than the join is worth (16, or 192 workgroups:
   // 1 x 8192, 32/8 of 128 in 64/32/24 pieces 20.0/15.9/15.0).
   const long items = static_cast<long>(a.num) * a.heads_kv;

