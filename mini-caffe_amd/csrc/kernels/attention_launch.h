@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 namespace mchip {
 namespace {
@@ -130,19 +131,32 @@ int launch_tiles(AttentionArgs a, hipStream_t st) {
 template <typename T, int DP, int RB>
 int launch_few_rows(AttentionArgs a, hipStream_t st) {
   using S = RowsShape<T, DP>;
-  // Pieces: enough for three rounds of workgroups (two or three to a CU, one where rows are
-  // wide), so that long and short contexts even out.  In bf16, with 3/4/6/8 times as many
-  // workgroups as CUs: 64 x 8192, 32/8 heads of 128 250/237/237/238 us; 10 x 20000, 16/2 of 64
-  // 23/22/24/31; 9 x 3089, 24/12 of 256 51/59/63/63.  But of two tiles per wavefront at least, or
-  // one where all are at work at once (1 x 513, 16/4 of 80 in fp16 9.1 us, two tiles 9.9; 16 x 1000, 32/8
-  // 19.4 and 16.0), and with few requests no more than the join is worth (16, or 192 workgroups:
-  // 1 x 8192, 32/8 of 128 in 64/32/24 pieces 20.0/15.9/15.0).
+  // The number of pieces that takes least time, counted in steps of a workgroup (a tile for each of
+  // its wavefronts; 1.2 us where rows are at most 256 bytes of 16-bit values): the longest piece, or
+  // what memory takes for all of them (180 workgroups' worth at once; lengths differ, so about half
+  // of max_context each), a little more where the CUs get unequal numbers of workgroups; the join,
+  // two trips past the L2 and the pieces' sums; the end, where the last pieces run alone; each
+  // workgroup's beginning.  us in 1/2/3/4/8/24 pieces, keys not in cache, 32/8 heads of 128 in bf16:
+  // 1 x 384 8.1/9.8/9.0, 1 x 5000 58/35/27/23/16/13.6; 16 x 512 13.0/13.9/13.9/15.0, up to 5000
+  // 69/48/57/52/53/56; 64 x 1000 52/57/59/62/76, up to 8192 245/228/223/223/226/241.  24/12 of 256, 7 x
+  // 1000: 34/26/25/33/36.
   const long items = static_cast<long>(a.num) * a.heads_kv;
   const int spans = std::max(1, ceil_div(a.max_context, S::kSpan));
-  const int shortest = items * spans <= 2 * kNumCu ? spans : (spans + 1) / 2;
-  const int most = std::min({shortest, kMaxPieces, static_cast<int>(std::max<long>(16, 192 / items))});
-  const int wanted =
-      static_cast<int>(std::min<long>(std::max<long>(1, (S::kRowBytes <= 256 ? 6 : 3) * kNumCu / items), most));
+  // (in steps, which take longer for wide rows and in fp32)
+  constexpr bool kShort = sizeof(T) == 2 && DP <= 128;
+  constexpr float kJoin = (kShort ? 700.f : sizeof(T) == 2 ? 450.f : 250.f) / S::kRowBytes;
+  constexpr float kBegin = kShort ? 0.5f : 0.9f;
+  const float sums = std::min<long>(static_cast<long>(a.max_q) * a.group.d, 16 * RB) * DP * 3e-4f;  // of one piece
+  int wanted = 1;
+  float best = 0.f;
+  for (const int pieces : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, kMaxPieces}) {
+    const int p = std::min(pieces, spans);
+    const float longest = static_cast<float>(ceil_div(spans, p)), per_cu = static_cast<float>(items * p) / kNumCu;
+    const float memory = static_cast<float>(items * spans) / 180.f * (0.8f + 0.2f * std::ceil(per_cu) / per_cu);
+    const float time = std::max(longest, memory) + (p > 1 ? kJoin + sums * p : 0.f) + 0.3f * longest + per_cu * kBegin;
+    if (p == 1 || time < best) best = time, wanted = p;
+    if (p == spans) break;
+  }
   a.piece = std::max(ceil_div(ceil_div(a.max_context, wanted), S::kSpan), 1) * S::kSpan;
   a.pieces = std::max(1, ceil_div(a.max_context, a.piece));
   if (a.pieces > 1) {

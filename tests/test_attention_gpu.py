@@ -713,3 +713,17 @@ def test_paged_many_chunks(A, kind, dim, block):
     keep = torch.ones(len(q), dtype=torch.bool, device="cuda")
     keep[mine] = False
     assert torch.equal(again[keep], out[keep]) and torch.equal(again_lse[:, keep], lse[:, keep])
+
+
+@pytest.mark.parametrize("kind,dim", [("f32", 64), ("bf16", 128), ("f16", 80), ("bf16", 256)])
+@pytest.mark.parametrize("requests,longest", [(1, 384), (1, 640), (5, 3000), (40, 700)])
+def test_paged_single_tokens_in_more_or_fewer_pieces(A, kind, dim, requests, longest):
+    """One piece, two, as many as there are steps; lengths far below the longest among them."""
+    g = torch.Generator(device="cuda").manual_seed(37)
+    contexts = [longest] + [1 + (97 * i) % longest for i in range(1, requests)]
+    keys, values, table, ks, vs = make_cache(g, contexts, 16, 2, dim, kind)
+    q = randn(g, requests, 6, dim, kind=kind)
+    first = paged(A, q, keys, values, table, [1] * requests, contexts)
+    check_paged(q, ks, vs, [1] * requests, contexts, *first)
+    again = paged(A, q, keys, values, table, [1] * requests, contexts)
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
